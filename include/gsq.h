@@ -356,6 +356,74 @@ int gsq_linear_allreduce(const void* w, int64_t row_bytes, int64_t rows, int ggm
 int gsq_peer_reduce_error_flag(int* flag);
 
 /*
+ * Mixture-of-experts layer over quantised experts, for a few tokens: y[t] = sum over the token's choices of
+ * weight * W2[e] q8(act(W13[e][gate] q8(x)) * (W13[e][up] q8(x))). Not in the reference's Route L (its stock path runs
+ * ggml_moe_a8 / ggml_moe_a8_vec, plugin/vllm_gguf_plugin/csrc/gguf/moe.cuh, moe_vec.cuh, with routing, activation and sum in
+ * kernels of their own; quantization/fused_moe.py). q8: 32 values to a 32-bit scale d = amax / 127, q = round(127 x / amax), ties away
+ * from zero; the quantised values are dotted as integers and scaled in fp32.
+ *
+ *   gsq_moe          the experts: w13 uint8 [experts, 2 * inter, bytes of `hidden` values], gate rows before up rows; w2 uint8
+ *                    [experts, hidden, bytes of `inter` values]; GGUF order (not repacked), any of the ten types each, 16-byte
+ *                    aligned; hidden and inter multiples of 256
+ *   x, y             [m, hidden] in x_dtype, rows x_row_stride / y_row_stride elements apart; y apart from x
+ *   topk_weights, topk_ids   [m, top_k] contiguous; ids int32, or int64 with ids_64 != 0. An id outside [0, experts) is a choice
+ *                    that is not here (another rank's): it adds nothing. A token without choices gets zeros. The same expert
+ *                    twice counts twice.
+ *   workspace        gsq_moe_workspace_bytes(...) bytes, 256-byte aligned; not initialised, not preserved; not to be shared by
+ *                    calls that may overlap
+ * gsq_moe_route: the choice alone. logits [m, experts] in `dtype`; scoring GSQ_MOE_SOFTMAX or _SIGMOID; the top_k largest
+ *   logits, or largest score + bias [experts] where bias is not NULL, ties to the lowest number; weight = score (divided by
+ *   the sum of the chosen ones where renormalize != 0) * scale. An expert with logit -inf or NaN is never chosen; a choice that
+ *   finds none left is id -1, weight 0. Experts at +inf share the weight.
+ * gsq_moe_layer: gsq_moe_route and gsq_moe_experts in one call, ids and weights kept in the workspace.
+ * Limits: experts <= 1024, top_k <= 32, m <= 65536 (GSQ_ERR_TOO_LARGE).
+ */
+#define GSQ_MOE_MAX_EXPERTS 1024
+#define GSQ_MOE_MAX_TOP_K 32
+#define GSQ_MOE_MAX_TOKENS 65536
+#define GSQ_ACT_SILU 0
+#define GSQ_ACT_GELU 1 /* g * Phi(g), by the error function */
+#define GSQ_MOE_SOFTMAX 0
+#define GSQ_MOE_SIGMOID 1
+typedef struct gsq_moe {
+  const void *w13, *w2;
+  int w13_type, w2_type;
+  int64_t experts, hidden, inter;
+  int activation;
+} gsq_moe;
+typedef struct gsq_moe_router {
+  const void* logits;
+  int dtype;
+  int64_t row_stride;
+  int scoring, renormalize;
+  const float* bias;
+  float scale;
+} gsq_moe_router;
+size_t gsq_moe_workspace_bytes(int64_t m, int64_t hidden, int64_t inter, int top_k);
+int gsq_moe_route(const gsq_moe_router* r, int64_t m, int64_t experts, int top_k, float* topk_weights, int32_t* topk_ids,
+                  void* stream);
+int gsq_moe_experts(const gsq_moe* w, const void* x, int x_dtype, int64_t m, int64_t x_row_stride, const float* topk_weights,
+                    const void* topk_ids, int ids_64, int top_k, void* y, int64_t y_row_stride, void* workspace,
+                    size_t workspace_bytes, void* stream);
+int gsq_moe_layer(const gsq_moe* w, const void* x, int x_dtype, int64_t m, int64_t x_row_stride, const gsq_moe_router* r, int top_k,
+                  void* y, int64_t y_row_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * What a server answers with behind the head: per row of logits [m, vocab] (dtype, rows row_stride elements apart) the log
+ * probability of one given token, its rank, the row's entropy and the top_n (0..32) most probable tokens with their log
+ * probabilities. Not in the reference (vLLM's sampler runs log_softmax, gather, a comparison and topk). Natural logarithms,
+ * statistics in fp32. Order of tokens: larger logit first, lower index first among equals, NaN last.
+ *   token_ids      [m] int64. Negative: no token (log probability 0, rank 0). >= vocab: NaN, rank 0.
+ *   logprobs [m], ranks [m] (1 = first in that order), entropy [m]
+ *   top_logprobs, top_ids   [m, top_n]; NULL where top_n = 0. Past the vocabulary: -inf, id -1.
+ * A masked logit (-inf) has probability 0 and log probability -inf; a row of only such has entropy 0. A NaN or +inf makes the
+ * row's log probabilities and entropy NaN (its order still holds).
+ */
+#define GSQ_LOGPROBS_MAX_TOP_N 32
+int gsq_token_logprobs(const void* logits, int dtype, int64_t m, int64_t vocab, int64_t row_stride, const int64_t* token_ids, int top_n,
+                       float* logprobs, int64_t* ranks, float* entropy, float* top_logprobs, int64_t* top_ids, void* stream);
+
+/*
  * Kernel family that serves (activation rows m, type, weight rows, k, packed) on B200: GSQ_KERNEL_*, the choice that
  * gsq_mul_mat_vec_q8 makes up to 8 activation rows and gsq_linear above (for the precision that is set, with
  * gsq_linear_workspace_bytes of scratch; a family that takes fewer rows per launch is launched several times). The op-level

@@ -1,0 +1,315 @@
+// Mixture-of-experts layer over GGUF-quantised experts for a few tokens (sm_100a): the router's choice, the 8-bit activations,
+// the host side. The products are in gsq_moe_dot.cu.
+//
+//   choice   s = softmax(logits) or sigmoid(logits); the top_k experts of largest logit (of largest s + bias where there is a
+//            bias), ties to the lowest number; weights s (/ their sum) * scale
+//   layer    y = sum over the choices of weight * W2[e] q8(act(W13[e][gate] q8(x)) * (W13[e][up] q8(x)))
+//
+// q8: 32 values to a 32-bit scale (moe_quant8). Sums in fp32; the activated product is rounded once, to its 8 bits, the result
+// once, to X's type. An expert whose logit is -inf or NaN is never chosen, and a choice that is not there (-1) adds nothing:
+// a token without experts gets zeros.
+#include "gsq_moe.cuh"
+
+namespace gsq {
+
+// Larger key = larger score; 0 = not to be chosen.
+__device__ __forceinline__ uint32_t score_key(float v) {
+  if (!(v > -INFINITY)) return 0;
+  const uint32_t b = __float_as_uint(v + 0.0f);   // (-0 and 0 are the same score)
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+__device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
+  return dtype == GSQ_F32 ? reinterpret_cast<const float*>(p)[i]
+         : dtype == GSQ_F16 ? __half2float(reinterpret_cast<const __half*>(p)[i])
+                            : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+}
+
+constexpr int ROUTE_PER_LANE = GSQ_MOE_MAX_EXPERTS / 32;
+
+struct RouteArgs {
+  const void* logits;
+  int dtype;
+  int64_t stride;
+  int m, experts, top_k, scoring, renormalize;
+  const float* bias;
+  float scale;
+  float* weights;
+  int32_t* ids;
+};
+
+// One warp, one token; lane l holds experts l, l + 32, ... Each round takes the largest key, the lowest number among equals.
+template <int PER_LANE>
+__device__ __forceinline__ void route_token(const RouteArgs& a, int token, int lane) {
+  float s[PER_LANE];
+  uint32_t key[PER_LANE];
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < PER_LANE; ++i) {
+    const int e = lane + 32 * i;
+    const float z = e < a.experts ? load_any(a.logits, a.dtype, token * a.stride + e) : -INFINITY;
+    s[i] = isnan(z) ? -INFINITY : fminf(z, 3.402823466e38f);   // experts at +inf share the weight
+    key[i] = score_key(s[i]);
+    top = fmaxf(top, s[i]);
+  }
+  float sum = 1.0f;
+  if (a.scoring == GSQ_MOE_SOFTMAX) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PER_LANE; ++i) {
+      s[i] = key[i] ? expf(s[i] - top) : 0.0f;
+      sum += s[i];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER_LANE; ++i) s[i] = key[i] ? __fdiv_rn(1.0f, 1.0f + expf(-s[i])) : 0.0f;
+  }
+  if (sum > 0.0f) {
+#pragma unroll
+    for (int i = 0; i < PER_LANE; ++i) s[i] = __fdiv_rn(s[i], sum);
+  }
+  if (a.bias) {
+#pragma unroll
+    for (int i = 0; i < PER_LANE; ++i)
+      if (key[i]) key[i] = score_key(s[i] + a.bias[lane + 32 * i]);
+  }
+  float mine = 0.0f, total = 0.0f;   // lane r keeps round r's choice
+  int id = -1;
+  for (int r = 0; r < a.top_k; ++r) {
+    uint32_t k = 0;
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < PER_LANE; ++i)
+      if (key[i] > k) {
+        k = key[i];
+        at = i;
+      }
+    const uint32_t best = __reduce_max_sync(0xFFFFFFFFu, k);
+    if (best == 0) break;
+    const uint32_t e = __reduce_min_sync(0xFFFFFFFFu, k == best ? (uint32_t)(lane + 32 * at) : 0xFFFFFFFFu);
+    float w = 0.0f;
+    const bool owner = (e & 31) == (uint32_t)lane;
+#pragma unroll
+    for (int i = 0; i < PER_LANE; ++i)
+      if (owner && i == (int)(e >> 5)) {
+        w = s[i];
+        key[i] = 0;
+      }
+    w = __shfl_sync(0xFFFFFFFFu, w, e & 31);
+    total += w;
+    if (lane == r) {
+      mine = w;
+      id = (int)e;
+    }
+  }
+  if (lane < a.top_k) {
+    if (a.renormalize) mine = total > 0.0f ? __fdiv_rn(mine, total) : 0.0f;
+    a.weights[(int64_t)token * a.top_k + lane] = mine * a.scale;
+    a.ids[(int64_t)token * a.top_k + lane] = id;
+  }
+}
+
+template <int PER_LANE>
+__global__ void __launch_bounds__(128) moe_route_kernel(const RouteArgs a) {
+  const int token = blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (token < a.m) route_token<PER_LANE>(a, token, threadIdx.x & 31);
+}
+
+static int launch_route(const RouteArgs& a, cudaStream_t st) {
+  const unsigned grid = (unsigned)((a.m + 3) / 4);
+  if (a.experts <= 64) moe_route_kernel<2><<<grid, 128, 0, st>>>(a);
+  else if (a.experts <= 256) moe_route_kernel<8><<<grid, 128, 0, st>>>(a);
+  else moe_route_kernel<ROUTE_PER_LANE><<<grid, 128, 0, st>>>(a);
+  GSQ_CUDA_TRY(cudaGetLastError());
+  return GSQ_OK;
+}
+
+// Rows of k values -> 8-bit form. One thread takes 8 values.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) moe_quant_kernel(const void* x, int64_t stride, int64_t rows, int k, int8_t* q8, float* d8) {
+  const int per_row = k >> 3;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / per_row;
+  const int c = (int)(i - row * per_row);
+  float v[8] = {};
+  if (row < rows) load8<T, VEC>(reinterpret_cast<const T*>(x), row * stride + 8 * c, v);
+  int q[8];
+  const float d = moe_quant8(v, q);
+  if (row < rows) {
+    *reinterpret_cast<uint2*>(q8 + row * k + 8 * c) = make_uint2(moe_pack4(q[0], q[1], q[2], q[3]), moe_pack4(q[4], q[5], q[6], q[7]));
+    if ((c & 3) == 0) d8[row * (k >> 5) + (c >> 2)] = d;
+  }
+}
+
+static int launch_quant(const void* x, int dtype, int vec, int64_t stride, int64_t rows, int k, int8_t* q8, float* d8, cudaStream_t st) {
+  const unsigned grid = (unsigned)((rows * (k >> 3) + 255) / 256);
+  if (dtype == GSQ_F32) {
+    if (vec) moe_quant_kernel<float, true><<<grid, 256, 0, st>>>(x, stride, rows, k, q8, d8);
+    else moe_quant_kernel<float, false><<<grid, 256, 0, st>>>(x, stride, rows, k, q8, d8);
+  } else if (dtype == GSQ_F16) {
+    if (vec) moe_quant_kernel<__half, true><<<grid, 256, 0, st>>>(x, stride, rows, k, q8, d8);
+    else moe_quant_kernel<__half, false><<<grid, 256, 0, st>>>(x, stride, rows, k, q8, d8);
+  } else {
+    if (vec) moe_quant_kernel<__nv_bfloat16, true><<<grid, 256, 0, st>>>(x, stride, rows, k, q8, d8);
+    else moe_quant_kernel<__nv_bfloat16, false><<<grid, 256, 0, st>>>(x, stride, rows, k, q8, d8);
+  }
+  GSQ_CUDA_TRY(cudaGetLastError());
+  return GSQ_OK;
+}
+
+// y = sum of a token's parts, in the order of its choices.
+__global__ void __launch_bounds__(256) moe_combine_kernel(const MoeArgs a) {
+  const int per_row = a.hidden >> 2;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, t = i / per_row;
+  if (t >= a.m) return;
+  const int c = 4 * (int)(i - t * per_row);
+  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int r = 0; r < a.top_k; ++r) {
+    const int64_t pair = t * a.top_k + r;
+    if (moe_expert(a, (int)pair) < 0) continue;
+    const float4 p = *reinterpret_cast<const float4*>(a.part + pair * a.hidden + c);
+    s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
+  }
+  const int64_t at = t * a.y_stride + c;
+  store_out_dyn(a.y, a.x_dtype, at, s.x);
+  store_out_dyn(a.y, a.x_dtype, at + 1, s.y);
+  store_out_dyn(a.y, a.x_dtype, at + 2, s.z);
+  store_out_dyn(a.y, a.x_dtype, at + 3, s.w);
+}
+
+// Workspace: pieces in the order of `next`, each 256-byte aligned.
+struct Pieces {
+  size_t at = 0;
+  size_t next(size_t bytes) {
+    const size_t p = at;
+    at += (bytes + 255) & ~(size_t)255;
+    return p;
+  }
+};
+struct MoeLayout {
+  size_t xq, xd, h, hq, hd, part, weights, ids, total;
+  MoeLayout(int64_t m, int64_t hidden, int64_t inter, int top_k) {
+    const size_t pairs = (size_t)m * top_k;
+    Pieces p;
+    xq = p.next((size_t)m * hidden);
+    xd = p.next((size_t)m * hidden / 8);
+    h = p.next(pairs * inter * 4);
+    hq = p.next(pairs * inter);
+    hd = p.next(pairs * inter / 8);
+    part = p.next(pairs * hidden * 4);
+    weights = p.next(pairs * 4);
+    ids = p.next(pairs * 4);
+    total = p.at;
+  }
+};
+
+static int check_router(const gsq_moe_router* r, int64_t m, int64_t experts, int top_k) {
+  if (!r || !r->logits || m < 0 || experts <= 0 || top_k <= 0 || top_k > experts || r->row_stride < 0) return GSQ_ERR_UNSUPPORTED;
+  if (experts > GSQ_MOE_MAX_EXPERTS || top_k > GSQ_MOE_MAX_TOP_K || m > INT32_MAX) return GSQ_ERR_TOO_LARGE;
+  if (r->dtype != GSQ_F32 && r->dtype != GSQ_F16 && r->dtype != GSQ_BF16) return GSQ_ERR_UNSUPPORTED;
+  if (r->scoring != GSQ_MOE_SOFTMAX && r->scoring != GSQ_MOE_SIGMOID) return GSQ_ERR_UNSUPPORTED;
+  return GSQ_OK;
+}
+
+static RouteArgs route_args(const gsq_moe_router* r, int64_t m, int64_t experts, int top_k, float* weights, int32_t* ids) {
+  return RouteArgs{r->logits, r->dtype, r->row_stride, (int)m, (int)experts, top_k, r->scoring, r->renormalize, r->bias, r->scale, weights, ids};
+}
+
+static int check_moe(const gsq_moe* w, const void* x, int x_dtype, int64_t m, int64_t x_row_stride, int top_k, const void* y,
+                     int64_t y_row_stride, const void* ws, size_t ws_bytes) {
+  if (!w || m < 0 || top_k <= 0 || w->experts <= 0) return GSQ_ERR_UNSUPPORTED;
+  const int b13 = block_bytes(w->w13_type), b2 = block_bytes(w->w2_type);
+  if (!b13 || !b2 || w->hidden <= 0 || w->inter <= 0 || w->hidden % 256 || w->inter % 256) return GSQ_ERR_UNSUPPORTED;
+  if (w->activation != GSQ_ACT_SILU && w->activation != GSQ_ACT_GELU) return GSQ_ERR_UNSUPPORTED;
+  if (x_dtype != GSQ_F32 && x_dtype != GSQ_F16 && x_dtype != GSQ_BF16) return GSQ_ERR_UNSUPPORTED;
+  if (m == 0) return GSQ_OK;
+  if (!w->w13 || !w->w2 || !x || !y || (uintptr_t)w->w13 % 16 || (uintptr_t)w->w2 % 16) return GSQ_ERR_UNSUPPORTED;
+  if (x_row_stride < 0 || (m > 1 && y_row_stride < w->hidden)) return GSQ_ERR_UNSUPPORTED;
+  if (w->hidden > (1 << 20) || w->inter > (1 << 20) || w->experts > GSQ_MOE_MAX_EXPERTS || top_k > GSQ_MOE_MAX_TOP_K || m > GSQ_MOE_MAX_TOKENS)
+    return GSQ_ERR_TOO_LARGE;
+  if (!ws || ws_bytes < gsq_moe_workspace_bytes(m, w->hidden, w->inter, top_k) || (uintptr_t)ws % 256) return GSQ_ERR_SCRATCH;
+  return GSQ_OK;
+}
+
+static int run_experts(const gsq_moe* w, const void* x, int x_dtype, int64_t m, int64_t x_row_stride, const float* weights, const void* ids,
+                       int ids64, int top_k, void* y, int64_t y_row_stride, uint8_t* ws, cudaStream_t st) {
+  const MoeLayout l(m, w->hidden, w->inter, top_k);
+  MoeArgs a;
+  a.w13 = (const uint8_t*)w->w13;
+  a.w2 = (const uint8_t*)w->w2;
+  a.rb13 = w->hidden / 256 * block_bytes(w->w13_type);
+  a.rb2 = w->inter / 256 * block_bytes(w->w2_type);
+  a.experts = (int)w->experts;
+  a.hidden = (int)w->hidden;
+  a.inter = (int)w->inter;
+  a.act = w->activation;
+  a.m = (int)m;
+  a.top_k = top_k;
+  a.x = x;
+  a.x_dtype = x_dtype;
+  a.x_stride = x_row_stride;
+  a.x_vec = (uintptr_t)x % 16 == 0 && (m == 1 || x_row_stride * (x_dtype == GSQ_F32 ? 4 : 2) % 16 == 0);
+  a.weights = weights;
+  a.ids = ids;
+  a.ids64 = ids64;
+  a.y = y;
+  a.y_stride = y_row_stride;
+  a.xq = (int8_t*)(ws + l.xq);
+  a.xd = (float*)(ws + l.xd);
+  a.h = (float*)(ws + l.h);
+  a.hq = (int8_t*)(ws + l.hq);
+  a.hd = (float*)(ws + l.hd);
+  a.part = (float*)(ws + l.part);
+  int rc = launch_quant(x, x_dtype, a.x_vec, x_row_stride, m, a.hidden, a.xq, a.xd, st);
+  if (rc == GSQ_OK) rc = moe_dot_gate_up(a, w->w13_type, st);
+  if (rc == GSQ_OK) rc = launch_quant(a.h, GSQ_F32, 1, a.inter, m * top_k, a.inter, a.hq, a.hd, st);
+  if (rc == GSQ_OK) rc = moe_dot_down(a, w->w2_type, st);
+  if (rc != GSQ_OK) return rc;
+  moe_combine_kernel<<<(unsigned)((m * (a.hidden >> 2) + 255) / 256), 256, 0, st>>>(a);
+  GSQ_CUDA_TRY(cudaGetLastError());
+  return GSQ_OK;
+}
+
+}  // namespace gsq
+
+extern "C" size_t gsq_moe_workspace_bytes(int64_t m, int64_t hidden, int64_t inter, int top_k) {
+  if (m <= 0 || hidden <= 0 || inter <= 0 || top_k <= 0) return 0;
+  return gsq::MoeLayout(m, hidden, inter, top_k).total;
+}
+
+extern "C" int gsq_moe_route(const gsq_moe_router* r, int64_t m, int64_t experts, int top_k, float* topk_weights, int32_t* topk_ids,
+                             void* stream) {
+  if (m == 0) return GSQ_OK;
+  const int rc = gsq::check_router(r, m, experts, top_k);
+  if (rc != GSQ_OK) return rc;
+  if (!topk_weights || !topk_ids) return GSQ_ERR_UNSUPPORTED;
+  return gsq::launch_route(gsq::route_args(r, m, experts, top_k, topk_weights, topk_ids), (cudaStream_t)stream);
+}
+
+extern "C" int gsq_moe_experts(const gsq_moe* w, const void* x, int x_dtype, int64_t m, int64_t x_row_stride, const float* topk_weights,
+                               const void* topk_ids, int ids_64, int top_k, void* y, int64_t y_row_stride, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  const int rc = gsq::check_moe(w, x, x_dtype, m, x_row_stride, top_k, y, y_row_stride, workspace, workspace_bytes);
+  if (rc != GSQ_OK || m == 0) return rc;
+  if (!topk_weights || !topk_ids) return GSQ_ERR_UNSUPPORTED;
+  return gsq::run_experts(w, x, x_dtype, m, x_row_stride, topk_weights, topk_ids, ids_64, top_k, y, y_row_stride, (uint8_t*)workspace,
+                          (cudaStream_t)stream);
+}
+
+extern "C" int gsq_moe_layer(const gsq_moe* w, const void* x, int x_dtype, int64_t m, int64_t x_row_stride, const gsq_moe_router* r, int top_k,
+                             void* y, int64_t y_row_stride, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = gsq::check_moe(w, x, x_dtype, m, x_row_stride, top_k, y, y_row_stride, workspace, workspace_bytes);
+  if (rc != GSQ_OK || m == 0) return rc;
+  rc = gsq::check_router(r, m, w->experts, top_k);
+  if (rc != GSQ_OK) return rc;
+  const gsq::MoeLayout l(m, w->hidden, w->inter, top_k);
+  uint8_t* ws = (uint8_t*)workspace;
+  float* weights = (float*)(ws + l.weights);
+  int32_t* ids = (int32_t*)(ws + l.ids);
+  rc = gsq::launch_route(gsq::route_args(r, m, w->experts, top_k, weights, ids), (cudaStream_t)stream);
+  if (rc != GSQ_OK) return rc;
+  return gsq::run_experts(w, x, x_dtype, m, x_row_stride, weights, ids, 0, top_k, y, y_row_stride, ws, (cudaStream_t)stream);
+}

@@ -427,6 +427,147 @@ std::tuple<Tensor, std::optional<Tensor>> silu_mul_quantize(const Tensor& gate_u
   return {q, y};
 }
 
+// ---- mixture-of-experts layer (gsq_b200.quantization.fused_moe) and log probabilities (gsq_b200.logprobs)
+
+// These ops have no backward pass: a call that would need one says so instead of returning a result without a gradient.
+void no_gradient(const char* op, std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : ts)
+    TORCH_CHECK(!t->defined() || !t->requires_grad(), op, ": no gradient is computed here; detach the input or call under torch.no_grad()");
+}
+
+gsq_moe moe_weights(const char* op, const Tensor& x, const Tensor& w13, const Tensor& w2, int64_t t13, int64_t t2, int64_t activation) {
+  TORCH_CHECK(quant_type(t13) && quant_type(t2), op, ": unsupported ggml type ", quant_type(t13) ? t2 : t13);
+  TORCH_CHECK(activation == GSQ_ACT_SILU || activation == GSQ_ACT_GELU, op, ": unknown activation ", activation);
+  TORCH_CHECK(x.dim() == 2, op, ": X must be 2-D");
+  TORCH_CHECK(dtype_code(x.scalar_type()) != GSQ_DTYPE_OTHER, op, ": X must be fp32, fp16 or bf16");
+  TORCH_CHECK(w13.dim() == 3 && w2.dim() == 3 && w13.size(0) == w2.size(0) && w13.size(0) > 0, op,
+              ": W13 and W2 must be [experts, rows, row bytes] of the same experts");
+  TORCH_CHECK(w13.scalar_type() == at::kByte && w2.scalar_type() == at::kByte, op, ": W13 and W2 must be uint8");
+  const int64_t hidden = x.size(1), inter = w13.size(1) / 2;
+  TORCH_CHECK(hidden > 0 && hidden % 256 == 0 && inter > 0 && inter % 256 == 0 && w13.size(1) == 2 * inter, op, ": hidden size ", hidden,
+              " and expert size ", w13.size(1), " / 2 must be multiples of 256");
+  TORCH_CHECK(w13.size(2) == hidden / 256 * gsq_type_block_bytes((int)t13), op, ": W13 rows of ", w13.size(2), " bytes do not hold ", hidden,
+              " values of type ", t13);
+  TORCH_CHECK(w2.size(1) == hidden && w2.size(2) == inter / 256 * gsq_type_block_bytes((int)t2), op, ": W2 must be [experts, ", hidden,
+              ", bytes of ", inter, " values of type ", t2, "]");
+  TORCH_CHECK(w13.is_contiguous() && w2.is_contiguous(), op, ": W13 and W2 must be contiguous");
+  TORCH_CHECK((uintptr_t)w13.const_data_ptr() % 16 == 0 && (uintptr_t)w2.const_data_ptr() % 16 == 0, op, ": W13 and W2 must be 16-byte aligned");
+  TORCH_CHECK(w13.size(0) <= GSQ_MOE_MAX_EXPERTS && x.size(0) <= GSQ_MOE_MAX_TOKENS, op, ": at most ", GSQ_MOE_MAX_EXPERTS, " experts and ",
+              GSQ_MOE_MAX_TOKENS, " tokens");
+  TORCH_CHECK(x.stride(1) == 1, op, ": X inner stride must be 1");
+  return {w13.const_data_ptr(), w2.const_data_ptr(), (int)t13, (int)t2, w13.size(0), hidden, inter, (int)activation};
+}
+
+void moe_on_device(const char* op, const Tensor& x, std::initializer_list<const Tensor*> ts) {
+  TORCH_CHECK(x.is_cuda(), op, ": X, the weights and the routing must be CUDA tensors");
+  for (const Tensor* t : ts) TORCH_CHECK(!t->defined() || t->device() == x.device(), op, ": all tensors must be on X's device");
+}
+
+gsq_moe_router moe_router(const char* op, const Tensor& logits, int64_t experts, int64_t top_k, int64_t scoring, bool renormalize,
+                          const Tensor& bias, double scale) {
+  TORCH_CHECK(logits.dim() == 2 && logits.size(1) == experts, op, ": router logits must be [tokens, ", experts, "]");
+  TORCH_CHECK(dtype_code(logits.scalar_type()) != GSQ_DTYPE_OTHER, op, ": router logits must be fp32, fp16 or bf16");
+  TORCH_CHECK(logits.stride(1) == 1 || experts == 1, op, ": router logits' inner stride must be 1");
+  TORCH_CHECK(top_k >= 1 && top_k <= experts && top_k <= GSQ_MOE_MAX_TOP_K, op, ": top_k=", top_k, " must be 1 .. min(experts, ",
+              GSQ_MOE_MAX_TOP_K, ")");
+  TORCH_CHECK(experts <= GSQ_MOE_MAX_EXPERTS && logits.size(0) <= INT32_MAX, op, ": at most ", GSQ_MOE_MAX_EXPERTS, " experts");
+  TORCH_CHECK(scoring == GSQ_MOE_SOFTMAX || scoring == GSQ_MOE_SIGMOID, op, ": unknown scoring ", scoring);
+  TORCH_CHECK(!bias.defined() || (bias.dim() == 1 && bias.size(0) == experts && bias.scalar_type() == at::kFloat && bias.is_contiguous()), op,
+              ": bias must be contiguous fp32 [", experts, "]");
+  return {logits.numel() ? logits.const_data_ptr() : nullptr, dtype_code(logits.scalar_type()), row_stride(logits, experts), (int)scoring, renormalize,
+          bias.defined() ? (const float*)bias.const_data_ptr() : nullptr, (float)scale};
+}
+
+Tensor moe_experts(const Tensor& x, const Tensor& w13, const Tensor& w2, const Tensor& topk_weights, const Tensor& topk_ids, int64_t t13,
+                   int64_t t2, int64_t activation) {
+  const char* op = "gsq_moe_experts";
+  const gsq_moe w = moe_weights(op, x, w13, w2, t13, t2, activation);
+  const int64_t m = x.size(0), top_k = topk_ids.dim() == 2 ? topk_ids.size(1) : 0;
+  TORCH_CHECK(topk_ids.dim() == 2 && topk_ids.size(0) == m && topk_weights.sizes() == topk_ids.sizes(), op,
+              ": topk_weights and topk_ids must be [", m, ", top_k]");
+  TORCH_CHECK(top_k >= 1 && top_k <= GSQ_MOE_MAX_TOP_K, op, ": top_k=", top_k, " must be 1 .. ", GSQ_MOE_MAX_TOP_K);
+  TORCH_CHECK(topk_ids.scalar_type() == at::kInt || topk_ids.scalar_type() == at::kLong, op, ": topk_ids must be int32 or int64");
+  TORCH_CHECK(topk_weights.is_floating_point(), op, ": topk_weights must be floating point");
+  no_gradient(op, {&x, &topk_weights});
+  moe_on_device(op, x, {&w13, &w2, &topk_weights, &topk_ids});
+  if (m == 0) return at::empty_like(x);
+  const c10::cuda::CUDAGuard dev(x.device());
+  const Tensor wt = topk_weights.to(at::kFloat).contiguous(), ids = topk_ids.contiguous();
+  const size_t need = gsq_moe_workspace_bytes(m, w.hidden, w.inter, (int)top_k);
+  Tensor y = result(m, w.hidden, x), ws = bytes((int64_t)need, x);
+  check(gsq_moe_experts(&w, x.const_data_ptr(), dtype_code(x.scalar_type()), m, row_stride(x, w.hidden), (const float*)wt.const_data_ptr(),
+                        ids.const_data_ptr(), ids.scalar_type() == at::kLong, (int)top_k, y.mutable_data_ptr(), y.stride(0), ws.mutable_data_ptr(),
+                        need, c10::cuda::getCurrentCUDAStream().stream()),
+        op);
+  return y;
+}
+
+Tensor moe_layer(const Tensor& x, const Tensor& logits, const Tensor& w13, const Tensor& w2, int64_t t13, int64_t t2, int64_t top_k,
+                 int64_t scoring, bool renormalize, const std::optional<Tensor>& bias, double scale, int64_t activation) {
+  const char* op = "gsq_moe_layer";
+  const gsq_moe w = moe_weights(op, x, w13, w2, t13, t2, activation);
+  const Tensor b = bias.value_or(Tensor());
+  const gsq_moe_router r = moe_router(op, logits, w.experts, top_k, scoring, renormalize, b, scale);
+  const int64_t m = x.size(0);
+  TORCH_CHECK(logits.size(0) == m, op, ": router logits of ", logits.size(0), " tokens, X has ", m);
+  no_gradient(op, {&x, &logits, &b});
+  moe_on_device(op, x, {&w13, &w2, &logits, &b});
+  if (m == 0) return at::empty_like(x);
+  const c10::cuda::CUDAGuard dev(x.device());
+  const size_t need = gsq_moe_workspace_bytes(m, w.hidden, w.inter, (int)top_k);
+  Tensor y = result(m, w.hidden, x), ws = bytes((int64_t)need, x);
+  check(gsq_moe_layer(&w, x.const_data_ptr(), dtype_code(x.scalar_type()), m, row_stride(x, w.hidden), &r, (int)top_k, y.mutable_data_ptr(),
+                      y.stride(0), ws.mutable_data_ptr(), need, c10::cuda::getCurrentCUDAStream().stream()),
+        op);
+  return y;
+}
+
+std::tuple<Tensor, Tensor> moe_route(const Tensor& logits, int64_t top_k, int64_t scoring, bool renormalize, const std::optional<Tensor>& bias,
+                                     double scale) {
+  const char* op = "gsq_moe_route";
+  const Tensor b = bias.value_or(Tensor());
+  TORCH_CHECK(logits.dim() == 2, op, ": router logits must be [tokens, experts]");
+  const int64_t m = logits.size(0), experts = logits.size(1);
+  const gsq_moe_router r = moe_router(op, logits, experts, top_k, scoring, renormalize, b, scale);
+  no_gradient(op, {&logits, &b});
+  moe_on_device(op, logits, {&b});
+  const c10::cuda::CUDAGuard dev(logits.device());
+  Tensor weights = at::empty({m, top_k}, logits.options().dtype(at::kFloat)), ids = at::empty({m, top_k}, logits.options().dtype(at::kInt));
+  if (m)
+    check(gsq_moe_route(&r, m, experts, (int)top_k, (float*)weights.mutable_data_ptr(), (int32_t*)ids.mutable_data_ptr(),
+                        c10::cuda::getCurrentCUDAStream().stream()),
+          op);
+  return {weights, ids};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits, const Tensor& token_ids, int64_t top_n) {
+  const char* op = "gsq_token_logprobs";
+  TORCH_CHECK(logits.dim() == 2 && logits.size(1) > 0, op, ": logits must be [rows, vocabulary]");
+  TORCH_CHECK(dtype_code(logits.scalar_type()) != GSQ_DTYPE_OTHER, op, ": logits must be fp32, fp16 or bf16");
+  const int64_t m = logits.size(0), vocab = logits.size(1);
+  TORCH_CHECK(logits.stride(1) == 1 || vocab == 1, op, ": logits' inner stride must be 1");
+  TORCH_CHECK(vocab <= (1 << 30), op, ": vocabulary too large");
+  TORCH_CHECK(token_ids.dim() == 1 && token_ids.size(0) == m, op, ": token_ids must be [", m, "]");
+  TORCH_CHECK(token_ids.scalar_type() == at::kInt || token_ids.scalar_type() == at::kLong, op, ": token_ids must be int32 or int64");
+  TORCH_CHECK(top_n >= 0 && top_n <= GSQ_LOGPROBS_MAX_TOP_N, op, ": top_n=", top_n, " must be 0 .. ", GSQ_LOGPROBS_MAX_TOP_N);
+  no_gradient(op, {&logits});
+  TORCH_CHECK(logits.is_cuda(), op, ": logits and token_ids must be CUDA tensors");
+  TORCH_CHECK(token_ids.device() == logits.device(), op, ": all tensors must be on the logits' device");
+  const c10::cuda::CUDAGuard dev(logits.device());
+  const Tensor ids = token_ids.to(at::kLong).contiguous();
+  const auto f32 = logits.options().dtype(at::kFloat), i64 = logits.options().dtype(at::kLong);
+  Tensor lp = at::empty({m}, f32), rank = at::empty({m}, i64), entropy = at::empty({m}, f32), top = at::empty({m, top_n}, f32),
+         top_ids = at::empty({m, top_n}, i64);
+  if (m)
+    check(gsq_token_logprobs(logits.const_data_ptr(), dtype_code(logits.scalar_type()), m, vocab, row_stride(logits, vocab),
+                             (const int64_t*)ids.const_data_ptr(), (int)top_n, (float*)lp.mutable_data_ptr(), (int64_t*)rank.mutable_data_ptr(),
+                             (float*)entropy.mutable_data_ptr(), top_n ? (float*)top.mutable_data_ptr() : nullptr,
+                             top_n ? (int64_t*)top_ids.mutable_data_ptr() : nullptr, c10::cuda::getCurrentCUDAStream().stream()),
+          op);
+  return {lp, rank, entropy, top, top_ids};
+}
+
 // ---- registration. The ops are defined in Python (which leaves names alone that another extension has defined); the
 // implementations are added here, one library object per (namespace, key) kept for the process's life.
 
@@ -463,6 +604,10 @@ void implement(const std::string& name) {
     else if (name == kSpec[Q6K_PACKED].name) l.impl(n, &op_self<Q6K_PACKED>);
     else if (name == "lcpp_quantize_q8_1") l.impl(n, &quantize_q8_1);
     else if (name == "gsq_linear_runs") l.impl(n, &linear_runs);
+    else if (name == "gsq_moe_experts") l.impl(n, &moe_experts);
+    else if (name == "gsq_moe_layer") l.impl(n, &moe_layer);
+    else if (name == "gsq_moe_route") l.impl(n, &moe_route);
+    else if (name == "gsq_token_logprobs") l.impl(n, &token_logprobs);
     else TORCH_CHECK(false, "no implementation of ", name);
   }
 }
@@ -486,6 +631,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         free_interpreter());
   m.def("rmsnorm_quantize", &rmsnorm_quantize, free_interpreter());
   m.def("silu_mul_quantize", &silu_mul_quantize, free_interpreter());
+  m.def("moe_experts", &moe_experts, free_interpreter());
+  m.def("moe_layer", &moe_layer, free_interpreter());
+  m.def("moe_route", &moe_route, free_interpreter());
+  m.def("token_logprobs", &token_logprobs, free_interpreter());
   m.def("route", [](int64_t n, int64_t type, int64_t rows, int64_t k, bool packed) -> std::optional<std::string> {
     const int op = route(n, type, rows, k, packed);
     return op < 0 ? std::nullopt : std::optional<std::string>(kSpec[op].name);

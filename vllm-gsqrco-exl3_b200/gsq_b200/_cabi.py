@@ -26,6 +26,7 @@ EXPORTS = (
     "gsq_debug_mmv_profile", "gsq_debug_mmv_max_rows", "gsq_debug_mmv_pdl", "gsq_debug_mmv_prefetch_first", "gsq_debug_mmv_chunking", "gsq_debug_mmv_trace",
     "gsq_linear", "gsq_linear_scratch_bytes", "gsq_linear_workspace_bytes", "gsq_debug_gemm_profile", "gsq_q6k_repack", "gsq_allreduce_sum", "gsq_allreduce_error_flag", "gsq_linear_allreduce", "gsq_peer_reduce_error_flag", "gsq_rmsnorm_quantize_q8_1", "gsq_silu_mul_quantize_q8_1", "gsq_dequantize_rows", "gsq_dequantize_bad_index_flag", "gsq_prefill_precision", "gsq_linear_vec",
     "gsq_linear_vec_pair", "gsq_linear_vec_pair_serves",
+    "gsq_moe_workspace_bytes", "gsq_moe_route", "gsq_moe_experts", "gsq_moe_layer", "gsq_token_logprobs",
 )
 
 
@@ -38,6 +39,18 @@ class PeerReduce(C.Structure):
 class Weight(C.Structure):
     """gsq_weight (include/gsq.h)."""
     _fields_ = [("w", C.c_void_p), ("row_bytes", C.c_int64), ("rows", C.c_int64), ("ggml_type", C.c_int), ("packed", C.c_int), ("y", C.c_void_p)]
+
+
+class Moe(C.Structure):
+    """gsq_moe (include/gsq.h)."""
+    _fields_ = [("w13", C.c_void_p), ("w2", C.c_void_p), ("w13_type", C.c_int), ("w2_type", C.c_int), ("experts", C.c_int64), ("hidden", C.c_int64),
+                ("inter", C.c_int64), ("activation", C.c_int)]
+
+
+class MoeRouter(C.Structure):
+    """gsq_moe_router (include/gsq.h)."""
+    _fields_ = [("logits", C.c_void_p), ("dtype", C.c_int), ("row_stride", C.c_int64), ("scoring", C.c_int), ("renormalize", C.c_int),
+                ("bias", C.c_void_p), ("scale", C.c_float)]
 
 
 class GuardArgs(C.Structure):
@@ -119,6 +132,16 @@ def _load() -> C.CDLL:
     lib.gsq_linear_vec_pair.argtypes = [C.POINTER(Weight), C.POINTER(Weight), vp, ci, i64, i64, i64, ci, i64, vp]
     lib.gsq_linear_vec_pair_serves.restype = ci
     lib.gsq_linear_vec_pair_serves.argtypes = [C.POINTER(Weight), C.POINTER(Weight), i64]
+    lib.gsq_moe_workspace_bytes.restype = sz
+    lib.gsq_moe_workspace_bytes.argtypes = [i64, i64, i64, ci]
+    lib.gsq_moe_route.restype = ci
+    lib.gsq_moe_route.argtypes = [C.POINTER(MoeRouter), i64, i64, ci, vp, vp, vp]
+    lib.gsq_moe_experts.restype = ci
+    lib.gsq_moe_experts.argtypes = [C.POINTER(Moe), vp, ci, i64, i64, vp, vp, ci, ci, vp, i64, vp, sz, vp]
+    lib.gsq_moe_layer.restype = ci
+    lib.gsq_moe_layer.argtypes = [C.POINTER(Moe), vp, ci, i64, i64, C.POINTER(MoeRouter), ci, vp, i64, vp, sz, vp]
+    lib.gsq_token_logprobs.restype = ci
+    lib.gsq_token_logprobs.argtypes = [vp, ci, i64, i64, i64, vp, ci, vp, vp, vp, vp, vp, vp]
     lib.gsq_iq3s_repack.restype = ci
     lib.gsq_iq3s_repack.argtypes = [vp, i64, i64, ci, vp]
     lib.gsq_allreduce_sum.restype = ci

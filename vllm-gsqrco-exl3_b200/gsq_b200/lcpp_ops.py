@@ -38,6 +38,12 @@ _SCHEMAS = {
     "gsq_mul_mat_q6k_packed": "(Tensor W, Tensor X, int type, SymInt row) -> Tensor",
     # nor this: a fused layer's runs of several types into one result (quantization/linear.py apply())
     "gsq_linear_runs": "(Tensor X, Tensor W, int[] runs, bool packed) -> Tensor",
+    # the mixture-of-experts layer (quantization/fused_moe.py) and the answer behind the head (logprobs.py)
+    "gsq_moe_experts": "(Tensor X, Tensor W13, Tensor W2, Tensor topk_weights, Tensor topk_ids, int w13_type, int w2_type, int activation) -> Tensor",
+    "gsq_moe_layer": "(Tensor X, Tensor logits, Tensor W13, Tensor W2, int w13_type, int w2_type, int top_k, int scoring, bool renormalize, "
+                     "Tensor? bias, float scale, int activation) -> Tensor",
+    "gsq_moe_route": "(Tensor logits, int top_k, int scoring, bool renormalize, Tensor? bias, float scale) -> (Tensor, Tensor)",
+    "gsq_token_logprobs": "(Tensor logits, Tensor token_ids, int top_n) -> (Tensor, Tensor, Tensor, Tensor, Tensor)",
 }
 
 
@@ -98,6 +104,20 @@ def _make_fake(name):
             (X.shape[0] * X.shape[1] // 128 * 144 if mmq else X.shape[0] * X.shape[1] // 32 * 36,), dtype=torch.uint8)
     if name == "gsq_linear_runs":
         return lambda X, W, runs, packed: X.new_empty((X.shape[0], sum(runs[1::4])))
+    if name == "gsq_moe_experts":
+        return lambda X, W13, W2, topk_weights, topk_ids, w13_type, w2_type, activation: X.new_empty(X.shape)
+    if name == "gsq_moe_layer":
+        return lambda X, logits, W13, W2, w13_type, w2_type, top_k, scoring, renormalize, bias, scale, activation: X.new_empty(X.shape)
+    if name == "gsq_moe_route":
+        return lambda logits, top_k, scoring, renormalize, bias, scale: (
+            logits.new_empty((logits.shape[0], top_k), dtype=torch.float32), logits.new_empty((logits.shape[0], top_k), dtype=torch.int32))
+    if name == "gsq_token_logprobs":
+        def fake(logits, token_ids, top_n):
+            m = logits.shape[0]
+            f32 = [logits.new_empty(s, dtype=torch.float32) for s in ((m,), (m,), (m, top_n))]
+            i64 = [logits.new_empty(s, dtype=torch.int64) for s in ((m,), (m, top_n))]
+            return f32[0], i64[0], f32[1], f32[2], i64[1]
+        return fake
     if "x_q8" in _SCHEMAS[name]:
         return lambda W, X, type, row, x_q8=None: X.new_empty((X.shape[0], row))
     return lambda W, X, type, row: X.new_empty((X.shape[0], row))
