@@ -56,27 +56,78 @@ __device__ __forceinline__ float ex2(float v) {
   return r;
 }
 
-// Sixteen bytes of logits.
+// Two fp32 numbers as one operand: half the issue slots of the scalar forms.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void halves(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// Sixteen bytes of logits. most(): the larger of two words' values, kept packed (the number where one side is NaN); floor():
+// values of at least LOWEST, NaN kept; larger(): `n` with the values > g counted in, to be read by total(); below(): the next
+// value under g.
 template <typename T>
 struct Vec;
 template <>
 struct Vec<float> {
   static constexpr int N = 4;
-  static __device__ __forceinline__ float most(const uint4& r) {
-    return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+  static constexpr float LOWEST = -1e38f, SMALL = -1e37f, LARGE = 1e37f;
+  static constexpr uint32_t MASKED = 0xFF800000u;     // -inf
+  static __device__ __forceinline__ uint32_t most(uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
+  static __device__ __forceinline__ float most(uint32_t a) { return __uint_as_float(a); }
+  static __device__ __forceinline__ uint32_t floor(uint32_t a) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(a)), "f"(LOWEST));
+    return __float_as_uint(r);
   }
   static __device__ __forceinline__ void get(const uint4& r, float (&f)[N]) {
     f[0] = __uint_as_float(r.x); f[1] = __uint_as_float(r.y); f[2] = __uint_as_float(r.z); f[3] = __uint_as_float(r.w);
   }
+  static __device__ __forceinline__ uint32_t larger(uint32_t n, const uint4& r, float g) {
+    float f[N];
+    get(r, f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) n += f[i] > g;
+    return n;
+  }
+  static __device__ __forceinline__ int total(uint32_t n) { return (int)n; }
+  static __device__ __forceinline__ float below(float g) { return nextafterf(g, -INFINITY); }
   static __device__ __forceinline__ float one(const float* p) { return *p; }
 };
+// The packed comparisons set all bits of a half. Subtracted from a 32-bit sum, such words leave the count L of the low halves in the
+// sum's low half and H - L in its high half, H the count of the high ones.
+__device__ __forceinline__ int packed_count(uint32_t n) { return (int)((2 * (n & 0xFFFFu) + (n >> 16)) & 0xFFFFu); }
 template <>
 struct Vec<__nv_bfloat16> {
   static constexpr int N = 8;
-  static __device__ __forceinline__ float most(const uint4& r) {   // (the packed maximum returns the number where one side is NaN)
-    const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&r);
-    const __nv_bfloat162 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
-    return fmaxf(__low2float(m), __high2float(m));
+  static constexpr float LOWEST = -1e38f, SMALL = -1e37f, LARGE = 1e37f;
+  static constexpr uint32_t MASKED = 0xFF80FF80u;
+  static __device__ __forceinline__ uint32_t most(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static __device__ __forceinline__ float most(uint32_t a) { return fmaxf(__uint_as_float(a << 16), __uint_as_float(a & 0xFFFF0000u)); }
+  static __device__ __forceinline__ uint32_t floor(uint32_t a) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(0xFE96FE96u));   // -9.97e37
+    return r;
   }
   static __device__ __forceinline__ void get(const uint4& r, float (&f)[N]) {
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
@@ -86,15 +137,38 @@ struct Vec<__nv_bfloat16> {
       f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
     }
   }
+  static __device__ __forceinline__ uint32_t larger(uint32_t n, const uint4& r, float g) {
+    const __nv_bfloat162 gg = __float2bfloat162_rn(g);
+    const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n -= __hgt2_mask(p[i], gg);
+    return n;
+  }
+  static __device__ __forceinline__ int total(uint32_t n) { return packed_count(n); }
+  static __device__ __forceinline__ float below(float g) {   // (of 0 and -0: the largest negative one)
+    const unsigned short b = __bfloat16_as_ushort(__float2bfloat16_rn(g));
+    return __bfloat162float(__ushort_as_bfloat16(g == 0.0f ? 0x8001 : g > 0.0f ? b - 1 : b + 1));
+  }
   static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 };
 template <>
 struct Vec<__half> {
   static constexpr int N = 8;
-  static __device__ __forceinline__ float most(const uint4& r) {
-    const __half2* p = reinterpret_cast<const __half2*>(&r);
-    const __half2 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
-    return fmaxf(__low2float(m), __high2float(m));
+  static constexpr float LOWEST = -65504.0f, SMALL = -6e4f, LARGE = 1e37f;
+  static constexpr uint32_t MASKED = 0xFC00FC00u;
+  static __device__ __forceinline__ uint32_t most(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static __device__ __forceinline__ float most(uint32_t a) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&a));
+    return fmaxf(v.x, v.y);
+  }
+  static __device__ __forceinline__ uint32_t floor(uint32_t a) {
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(0xFBFFFBFFu));   // -65504
+    return r;
   }
   static __device__ __forceinline__ void get(const uint4& r, float (&f)[N]) {
     const __half2* p = reinterpret_cast<const __half2*>(&r);
@@ -104,6 +178,18 @@ struct Vec<__half> {
       f[2 * i] = v.x;
       f[2 * i + 1] = v.y;
     }
+  }
+  static __device__ __forceinline__ uint32_t larger(uint32_t n, const uint4& r, float g) {
+    const __half2 gg = __float2half2_rn(g);
+    const __half2* p = reinterpret_cast<const __half2*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n -= __hgt2_mask(p[i], gg);
+    return n;
+  }
+  static __device__ __forceinline__ int total(uint32_t n) { return packed_count(n); }
+  static __device__ __forceinline__ float below(float g) {   // (of 0 and -0: the largest negative one)
+    const unsigned short b = __half_as_ushort(__float2half_rn(g));
+    return __half2float(__ushort_as_half(g == 0.0f ? 0x8001 : g > 0.0f ? b - 1 : b + 1));
   }
   static __device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
 };
@@ -128,22 +214,76 @@ __device__ __forceinline__ Stat join(Stat a, Stat b) {
   return Stat{m, a.s + b.s, a.t + b.t};
 }
 
-// The values of one thread's vectors go through here. `most`: their maximum.
-template <int N>
-__device__ __forceinline__ void add_values(Stat& a, const float (&f)[N], float most) {
-  if (most > -INFINITY) {
-    raise(a, most);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {              // (x log2 e - m log2 e in one step would overflow at the types' lowest values)
-      const float y = (f[i] - a.m) * LOG2E, e = ex2(y);
-      a.s += e;
-      a.t = fmaf(e, fmaxf(y, -1e4f), a.t);     // (0 times -inf of a masked value)
-    }
-  } else {                                     // -inf and NaN only
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (isnan(f[i])) a.s = NAN;
+// The parts of n lanes (a power of two; lanes n, n + 1, ... hold lane 0's, 1's, ... again) in one order.
+__device__ __forceinline__ void join_parts(Stat st, int before, int n, Stat* to, int* to_before) {
+  const int lane = threadIdx.x & 31;
+  for (int o = n >> 1; o > 0; o >>= 1) {
+    const Stat b{__shfl_xor_sync(0xFFFFFFFFu, st.m, o), __shfl_xor_sync(0xFFFFFFFFu, st.s, o), __shfl_xor_sync(0xFFFFFFFFu, st.t, o)};
+    st = lane & o ? join(b, st) : join(st, b);
+    before += __shfl_xor_sync(0xFFFFFFFFu, before, o);
   }
+  if (lane == 0) {
+    *to = st;
+    *to_before = before;
+  }
+}
+
+// One value.
+__device__ __forceinline__ void add_value(Stat& a, float f) {
+  if (f > -INFINITY) {
+    raise(a, f);
+    const float y = (f - a.m) * LOG2E, e = ex2(y);
+    a.s += e;
+    a.t = fmaf(e, fmaxf(y, -1e4f), a.t);       // (0 times -inf)
+  } else if (isnan(f)) {
+    a.s = NAN;
+  }
+}
+
+// U vectors of one thread; returns their maximum. One comparison decides for all of them whether the sums are rescaled. A masked
+// value (-inf) is taken as LOWEST, whose exponential is 0 as well and 0 times whose distance stays 0, as long as the maximum is
+// far from LOWEST and from overflow; where it is not, the values go one by one.
+template <typename T, int U>
+__device__ __forceinline__ float add_vectors(Stat& a, const uint4 (&r)[U]) {
+  using V = Vec<T>;
+  uint32_t top = r[0].x;
+#pragma unroll
+  for (int u = 0; u < U; ++u) top = V::most(top, V::most(V::most(r[u].x, r[u].y), V::most(r[u].z, r[u].w)));
+  const float most = V::most(top);
+  if (most > -INFINITY) raise(a, most);
+  if (a.m > V::SMALL && a.m < V::LARGE) {
+    const uint64_t shift = pair(-a.m, -a.m), scale = pair(LOG2E, LOG2E);
+    uint64_t s[2] = {0, 0}, t[2] = {0, 0};     // (two chains each)
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint4 w = make_uint4(V::floor(r[u].x), V::floor(r[u].y), V::floor(r[u].z), V::floor(r[u].w));
+      float f[V::N];
+      V::get(w, f);
+#pragma unroll
+      for (int i = 0; i < V::N; i += 2) {      // (x log2 e - m log2 e in one step would be off by more where both are large)
+        const uint64_t y = mul2(add2(pair(f[i], f[i + 1]), shift), scale);
+        float y0, y1;
+        halves(y, y0, y1);
+        const uint64_t e = pair(ex2(y0), ex2(y1));
+        s[(i >> 1) & 1] = add2(s[(i >> 1) & 1], e);
+        t[(i >> 1) & 1] = fma2(e, y, t[(i >> 1) & 1]);
+      }
+    }
+    float s0, s1, t0, t1;
+    halves(add2(s[0], s[1]), s0, s1);
+    halves(add2(t[0], t[1]), t0, t1);
+    a.s += s0 + s1;
+    a.t += t0 + t1;
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float f[V::N];
+      V::get(r[u], f);
+#pragma unroll
+      for (int i = 0; i < V::N; ++i) add_value(a, f[i]);
+    }
+  }
+  return most;
 }
 
 struct LogprobShared {
@@ -151,10 +291,10 @@ struct LogprobShared {
   unsigned long long best[GSQ_LOGPROBS_MAX_TOP_N];   // this block's alternatives in order; 0 past the last
   Stat stat[LP_WARPS];
   int before[LP_WARPS];
-  Stat part;                                         // the block's: read by the cluster's first block
+  Stat part;                                         // the block's: read by the cluster's first block; there, then the row's
   int part_before;
   float group[32];
-  float limit;
+  unsigned long long least;
   int found, hot_found, scan[LP_WARPS];
   uint16_t hot[LP_THREADS];
 };
@@ -275,18 +415,15 @@ __device__ void alternatives(LogprobShared& sh, const Part<T>& p, float mine, in
   for (int o = LP_THREADS / 64; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
   if (tid % (LP_THREADS / 32) == 0) sh.group[tid / (LP_THREADS / 32)] = g;
   __syncthreads();
-  if (tid < 32) {
-    g = sh.group[lane];
-    int place = 0;
+  g = sh.group[lane];
+  int place = 0;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      const float v = __shfl_sync(0xFFFFFFFFu, g, j);
-      place += v > g || (v == g && j < lane);
-    }
-    if (place == top_n - 1) sh.limit = g;
+  for (int j = 0; j < 32; ++j) {
+    const float v = __shfl_sync(0xFFFFFFFFu, g, j);
+    place += v > g || (v == g && j < lane);
   }
-  __syncthreads();
-  float limit = sh.limit;
+  const uint32_t at = __ballot_sync(0xFFFFFFFFu, place == top_n - 1);
+  float limit = __shfl_sync(0xFFFFFFFFu, g, __ffs(at) - 1);
   int found = collect(sh, p, mine, limit, true);
   if (found > LP_ROOM) {
     // more than the list takes reach the limit: the larger ones, with a limit that rises to the top_n-th of those seen until
@@ -307,6 +444,36 @@ __device__ void alternatives(LogprobShared& sh, const Part<T>& p, float mine, in
     take_in_order(sh, p, top_n - found, [](float v) { return isnan(v); });
   }
   order_list(sh, sh.cand, sh.found, sh.best, top_n);
+}
+
+// The blocks' lists (each in order) into sh.cand, but for what cannot be among the first top_n: 32 keys, the first 32 / cs of
+// every list, have a top_n-th largest; smaller ones are left out.
+__device__ __forceinline__ void join_lists(LogprobShared& sh, cg::cluster_group& cluster, int cs, int top_n) {
+  const int tid = threadIdx.x;
+  unsigned long long k[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {                   // cs * top_n <= 512
+    const int i = tid + j * LP_THREADS;
+    k[j] = i < cs * top_n ? cluster.map_shared_rank(&sh, i / top_n)->best[i % top_n] : 0;
+  }
+  if (tid < 32) {
+    const int per = 32 / cs;
+    const unsigned long long g = tid % per < top_n ? cluster.map_shared_rank(&sh, tid / per)->best[tid % per] : 0;
+    int place = 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const unsigned long long v = __shfl_sync(0xFFFFFFFFu, g, j);
+      place += v > g || (v == g && j < tid);
+    }
+    if (place == top_n - 1) sh.least = g;
+    if (tid == 0) sh.found = 0;
+  }
+  __syncthreads();
+  const unsigned long long least = sh.least;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    if (k[j] && k[j] >= least) sh.cand[atomicAdd(&sh.found, 1)] = k[j];
+  __syncthreads();
 }
 
 template <typename T>
@@ -331,56 +498,64 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobAr
   p.v1 = (int)((int64_t)vectors * (rank + 1) / cs);
 
   // the first loads are on their way before the given token is looked up
-  uint4 next[LP_UNROLL];
+  constexpr int U = LP_UNROLL;
+  uint4 next[U];
   auto fetch = [&](int v) {
+    if (v + (U - 1) * LP_THREADS < p.v1) {
 #pragma unroll
-    for (int u = 0; u < LP_UNROLL; ++u)
-      if (v + u * LP_THREADS < p.v1) next[u] = ldg_stream_v4(p.body + (int64_t)(v + u * LP_THREADS) * N);
+      for (int u = 0; u < U; ++u) next[u] = ldg_stream_v4(p.body + (int64_t)(v + u * LP_THREADS) * N);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        next[u] = make_uint4(Vec<T>::MASKED, Vec<T>::MASKED, Vec<T>::MASKED, Vec<T>::MASKED);
+        if (v + u * LP_THREADS < p.v1) next[u] = ldg_stream_v4(p.body + (int64_t)(v + u * LP_THREADS) * N);
+      }
+    }
   };
   fetch(p.v0 + tid);
   const int64_t id64 = a.ids[row];
   const bool has = id64 >= 0 && id64 < a.vocab;
   const int id = has ? (int)id64 : -1;
   const float given = has ? Vec<T>::one(p.row + id) : INFINITY;
-  const bool odd = isnan(given);                              // its place is behind every number
   const unsigned long long given_key = lp_key(given, id);
-
+  // values in front of the given one: larger ones, and equal ones of vectors that end before it (those of its own vector are added
+  // below). A masked or NaN one has no value under it: keys are compared one by one.
+  const bool odd = has && !(given > -INFINITY);
+  const float under = Vec<T>::below(given);
+  const int own = has && id >= p.body_at ? (id - p.body_at) / N : -1;   // the given token's vector
   Stat st{-INFINITY, 0.0f, 0.0f};
   int before = 0;
-  // values in front of the given one: those of a vector that lies before it count when equal too
-  auto count = [&](const float (&f)[N], int at) {
-    if (odd || (at <= id && id < at + N)) {
+  for (int v = p.v0 + tid; v < p.v1; v += U * LP_THREADS) {
+    uint4 now[U];
 #pragma unroll
-      for (int i = 0; i < N; ++i) before += lp_key(f[i], at + i) > given_key;
-    } else if (at < id) {
+    for (int u = 0; u < U; ++u) now[u] = next[u];
+    fetch(v + U * LP_THREADS);
+    const float most = add_vectors<T, U>(st, now);
+    if (has && !odd && most >= given) {
+      uint32_t n = 0;
 #pragma unroll
-      for (int i = 0; i < N; ++i) before += f[i] >= given;
-    } else {
+      for (int u = 0; u < U; ++u) n = Vec<T>::larger(n, now[u], v + u * LP_THREADS < own ? under : given);
+      before += Vec<T>::total(n);
+    } else if (odd) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) before += f[i] > given;
-    }
-  };
-  for (int v = p.v0 + tid; v < p.v1; v += LP_UNROLL * LP_THREADS) {
-    uint4 now[LP_UNROLL];
-#pragma unroll
-    for (int u = 0; u < LP_UNROLL; ++u) now[u] = next[u];
-    fetch(v + LP_UNROLL * LP_THREADS);
-#pragma unroll
-    for (int u = 0; u < LP_UNROLL; ++u) {
-      if (v + u * LP_THREADS < p.v1) {
-        const float most = Vec<T>::most(now[u]);
+      for (int u = 0; u < U; ++u) {
         float f[N];
         Vec<T>::get(now[u], f);
-        add_values<N>(st, f, most);
-        if (has && (most >= given || odd)) count(f, p.body_at + (v + u * LP_THREADS) * N);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          before += v + u * LP_THREADS < p.v1 && lp_key(f[i], p.body_at + (v + u * LP_THREADS) * N + i) > given_key;
       }
     }
   }
+  if (!odd && has && own >= p.v0 && own < p.v1 && tid < N) {
+    const int i = p.body_at + own * N + tid;
+    before += i < id && Vec<T>::one(p.row + i) == given;
+  }
   if ((tid < p.head) || (tid >= 32 && tid - 32 < p.tail)) {   // single values at the row's ends
     const int i = tid < 32 ? tid : p.tail_at + tid - 32;
-    const float f[1] = {Vec<T>::one(p.row + i)};
-    add_values<1>(st, f, isnan(f[0]) ? -INFINITY : f[0]);
-    before += has && lp_key(f[0], i) > given_key;
+    const float f = Vec<T>::one(p.row + i);
+    add_value(st, f);
+    before += has && lp_key(f, i) > given_key;
   }
   const float mine = st.m;
 
@@ -396,26 +571,21 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobAr
   }
   if (a.top_n) alternatives(sh, p, mine, a.top_n);
   else __syncthreads();
-  if (tid == 0) {
-    st = sh.stat[0];
-    before = sh.before[0];
-    for (int w = 1; w < LP_WARPS; ++w) {
-      st = join(st, sh.stat[w]);
-      before += sh.before[w];
+  if (tid < 32) join_parts(sh.stat[lane & (LP_WARPS - 1)], sh.before[lane & (LP_WARPS - 1)], LP_WARPS, &sh.part, &sh.part_before);
+  if (cs > 1) {
+    cluster.sync();
+    if (rank == 0 && tid < 32) {
+      const LogprobShared* q = cluster.map_shared_rank(&sh, lane & (cs - 1));
+      const Stat part = q->part;
+      const int part_before = q->part_before;
+      __syncwarp();
+      join_parts(part, part_before, cs, &sh.part, &sh.part_before);
     }
-    sh.part = st;
-    sh.part_before = before;
   }
-  if (cs > 1) cluster.sync();
-  else __syncthreads();
   if (rank == 0) {
+    __syncthreads();
     st = sh.part;
     before = sh.part_before;
-    for (int r = 1; r < cs; ++r) {
-      const LogprobShared* q = cluster.map_shared_rank(&sh, r);
-      st = join(st, q->part);
-      before += q->part_before;
-    }
     const float base = st.m == -INFINITY ? 0.0f : st.m, lse = logf(st.s);
     auto logprob = [&](float v) { return v == -INFINITY && !isnan(lse) ? -INFINITY : (v - base) - lse; };
     if (tid == 0) {
@@ -426,10 +596,9 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobAr
     if (a.top_n) {
       const unsigned long long* best = sh.best;
       if (cs > 1) {                               // the blocks' lists, joined
-        for (int i = tid; i < cs * a.top_n; i += LP_THREADS) sh.cand[i] = cluster.map_shared_rank(&sh, i / a.top_n)->best[i % a.top_n];
-        __syncthreads();
+        join_lists(sh, cluster, cs, a.top_n);
         unsigned long long* joined = sh.cand + 16 * GSQ_LOGPROBS_MAX_TOP_N;
-        order_list(sh, sh.cand, cs * a.top_n, joined, a.top_n);
+        order_list(sh, sh.cand, sh.found, joined, a.top_n);
         best = joined;
       }
       if (tid < a.top_n) {
