@@ -36,6 +36,7 @@ constexpr int LP_THREADS = 256;
 constexpr int LP_WARPS = LP_THREADS / 32;
 constexpr int LP_UNROLL = 4;      // 16-byte loads of a thread in flight, twice
 constexpr int LP_ROOM = 1024;     // candidates of a block
+constexpr int LP_AGAIN = 512;     // rounds of one thread to be read again
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.69314718055994531f;
 
 // Order of a row: larger key first. High half: the value (NaN 0, then -inf up); low half: lower index, larger key.
@@ -295,8 +296,8 @@ struct LogprobShared {
   int part_before;
   float group[32];
   unsigned long long least;
-  int found, hot_found, scan[LP_WARPS];
-  uint16_t hot[LP_THREADS];
+  int found, again_found, scan[LP_WARPS];
+  uint32_t again[LP_AGAIN];                          // vectors (of the part) at which a thread's round to be read again begins
 };
 
 // The part of a row that a block has: `head` single values, whole vectors [v0, v1), `tail` single values, in index order.
@@ -358,31 +359,42 @@ __device__ void take_in_order(LogprobShared& sh, const Part<T>& p, int need, P p
   __syncthreads();
 }
 
+// What a thread remembers of its rounds of loads: the largest maximum of one, which it was, and the largest of the others.
+struct Rounds {
+  float most, second;
+  int at;
+};
+
 // The block's values that are larger than `limit` (or equal: `equal`) into the list; returns how many there are, of which the
-// first LP_ROOM are in it. `mine`: the calling thread's maximum.
+// first LP_ROOM are in it. Only rounds whose maximum reaches the limit are read again: mostly one of a few threads each.
 template <typename T>
-__device__ int collect(LogprobShared& sh, const Part<T>& p, float mine, float limit, bool equal) {
+__device__ int collect(LogprobShared& sh, const Part<T>& p, const Rounds& mine, int rounds, float limit, bool equal) {
   const int tid = threadIdx.x;
-  if (tid == 0) sh.found = sh.hot_found = 0;
+  if (tid == 0) sh.found = sh.again_found = 0;
   __syncthreads();
-  if (equal ? mine >= limit : mine > limit) sh.hot[atomicAdd(&sh.hot_found, 1)] = (uint16_t)tid;
+  auto reaches = [&](float v) { return equal ? v >= limit : v > limit; };
+  if (reaches(mine.most)) {
+    const int n = reaches(mine.second) ? rounds : 1, at = atomicAdd(&sh.again_found, n);
+    for (int i = 0; i < n; ++i)
+      if (at + i < LP_AGAIN) sh.again[at + i] = (n == 1 ? mine.at : i) * (LP_UNROLL * LP_THREADS) + tid;
+  }
   __syncthreads();
-  const int per = (p.v1 - p.v0 + LP_THREADS - 1) / LP_THREADS, tasks = sh.hot_found * per + 2;
+  const int again = sh.again_found, vectors = p.v1 - p.v0;
+  const bool all = again > LP_AGAIN;              // every vector of the part
+  const int tasks = 2 + (all ? vectors : again * LP_UNROLL);
   for (int j = tid; j < tasks; j += LP_THREADS) {
-    int u;                                        // the edges, then every vector of the hot threads
-    if (j < 2) {
-      u = j == 0 ? 0 : p.v1 - p.v0 + 1;
-    } else {
-      const int h = (j - 2) / per;
-      u = 1 + sh.hot[h] + ((j - 2) - h * per) * LP_THREADS;
-      if (u > p.v1 - p.v0) continue;
+    int u = j == 0 ? 0 : vectors + 1;             // the edges first
+    if (j >= 2) {
+      const int v = all ? j - 2 : (int)sh.again[(j - 2) / LP_UNROLL] + (j - 2) % LP_UNROLL * LP_THREADS;
+      if (v >= vectors) continue;
+      u = v + 1;
     }
     float f[Vec<T>::N];
     int at;
     const int n = p.unit(u, f, at);
 #pragma unroll
     for (int i = 0; i < Vec<T>::N; ++i)
-      if (i < n && (equal ? f[i] >= limit : f[i] > limit)) {
+      if (i < n && reaches(f[i])) {
         const int slot = atomicAdd(&sh.found, 1);
         if (slot < LP_ROOM) sh.cand[slot] = lp_key(f[i], at + i);
       }
@@ -408,7 +420,7 @@ __device__ __forceinline__ void order_list(LogprobShared& sh, const unsigned lon
 
 // The block's top_n alternatives, in order, into sh.best.
 template <typename T>
-__device__ void alternatives(LogprobShared& sh, const Part<T>& p, float mine, int top_n) {
+__device__ void alternatives(LogprobShared& sh, const Part<T>& p, float mine, const Rounds& mine_by_round, int rounds, int top_n) {
   const int tid = threadIdx.x, lane = tid & 31;
   float g = mine;
 #pragma unroll
@@ -424,15 +436,15 @@ __device__ void alternatives(LogprobShared& sh, const Part<T>& p, float mine, in
   }
   const uint32_t at = __ballot_sync(0xFFFFFFFFu, place == top_n - 1);
   float limit = __shfl_sync(0xFFFFFFFFu, g, __ffs(at) - 1);
-  int found = collect(sh, p, mine, limit, true);
+  int found = collect(sh, p, mine_by_round, rounds, limit, true);
   if (found > LP_ROOM) {
     // more than the list takes reach the limit: the larger ones, with a limit that rises to the top_n-th of those seen until
     // they fit (it rises to a value that is larger than the last one), then the equal ones of lowest index
-    found = collect(sh, p, mine, limit, false);
+    found = collect(sh, p, mine_by_round, rounds, limit, false);
     while (found > LP_ROOM) {
       order_list(sh, sh.cand, LP_ROOM, sh.best, top_n);
       limit = lp_key_value(sh.best[top_n - 1]);
-      found = collect(sh, p, mine, limit, false);
+      found = collect(sh, p, mine_by_round, rounds, limit, false);
     }
     if (found < top_n) take_in_order(sh, p, top_n - found, [limit](float v) { return v == limit; });
   }
@@ -525,12 +537,19 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobAr
   const int own = has && id >= p.body_at ? (id - p.body_at) / N : -1;   // the given token's vector
   Stat st{-INFINITY, 0.0f, 0.0f};
   int before = 0;
-  for (int v = p.v0 + tid; v < p.v1; v += U * LP_THREADS) {
+  const int rounds = (p.v1 - p.v0 + U * LP_THREADS - 1) / (U * LP_THREADS);
+  Rounds by_round{-INFINITY, -INFINITY, 0};
+  for (int round = 0, v = p.v0 + tid; v < p.v1; ++round, v += U * LP_THREADS) {
     uint4 now[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) now[u] = next[u];
     fetch(v + U * LP_THREADS);
     const float most = add_vectors<T, U>(st, now);
+    by_round.second = fmaxf(by_round.second, fminf(most, by_round.most));
+    if (most > by_round.most) {
+      by_round.most = most;
+      by_round.at = round;
+    }
     if (has && !odd && most >= given) {
       uint32_t n = 0;
 #pragma unroll
@@ -569,7 +588,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobAr
     sh.stat[tid >> 5] = st;
     sh.before[tid >> 5] = before;
   }
-  if (a.top_n) alternatives(sh, p, mine, a.top_n);
+  if (a.top_n) alternatives(sh, p, mine, by_round, rounds, a.top_n);
   else __syncthreads();
   if (tid < 32) join_parts(sh.stat[lane & (LP_WARPS - 1)], sh.before[lane & (LP_WARPS - 1)], LP_WARPS, &sh.part, &sh.part_before);
   if (cs > 1) {
@@ -611,8 +630,130 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobAr
   if (cs > 1) cluster.sync();                     // no block leaves while its part may be read
 }
 
+// Rows of at most 256 whole vectors: a warp a row, the row in registers, no barrier. With a block a row, 4096 rows of 1000 fp32 logits
+// took 46 us: a row's fixed steps outweigh its 4 KB.
+constexpr int LPW_WARPS = 8, LPW_VECTORS = 8, LPW_ROOM = 128;
+
+template <typename T>
+__global__ void __launch_bounds__(LPW_WARPS * 32) logprobs_rows_kernel(const LogprobArgs a, int rows) {
+  constexpr int N = Vec<T>::N, H = LPW_VECTORS / 2;
+  __shared__ unsigned long long cand_all[LPW_WARPS][LPW_ROOM], best_all[LPW_WARPS][GSQ_LOGPROBS_MAX_TOP_N];
+  __shared__ int found_all[LPW_WARPS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * LPW_WARPS + warp;
+  if (row >= rows) return;
+  const T* x = reinterpret_cast<const T*>(a.x) + row * a.stride;
+  const int head = min(a.vocab, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T));
+  const int vectors = (a.vocab - head) / N, tail_at = head + vectors * N;
+  uint4 r[2][H];
+#pragma unroll
+  for (int u = 0; u < LPW_VECTORS; ++u) {
+    r[u / H][u % H] = make_uint4(Vec<T>::MASKED, Vec<T>::MASKED, Vec<T>::MASKED, Vec<T>::MASKED);
+    if (lane + 32 * u < vectors) r[u / H][u % H] = ldg_stream_v4(x + head + (lane + 32 * u) * N);
+  }
+  const int64_t id64 = a.ids[row];
+  // a lane's single value: of the head (lanes 0 ..) or of the tail (lanes 16 ..)
+  const int single = lane < head ? lane : lane >= 16 && tail_at + lane - 16 < a.vocab ? tail_at + lane - 16 : -1;
+  const float edge = single >= 0 ? Vec<T>::one(x + single) : 0.0f;
+  const bool has = id64 >= 0 && id64 < a.vocab;
+  const int id = has ? (int)id64 : -1;
+  const float given = has ? Vec<T>::one(x + id) : INFINITY;
+  const unsigned long long given_key = lp_key(given, id);
+  // every value of the lane and its index
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int u = 0; u < LPW_VECTORS; ++u) {
+      if (lane + 32 * u < vectors) {
+        float v[N];
+        Vec<T>::get(r[u / H][u % H], v);
+#pragma unroll
+        for (int i = 0; i < N; ++i) f(v[i], head + (lane + 32 * u) * N + i);
+      }
+    }
+    if (single >= 0) f(edge, single);
+  };
+  Stat st{-INFINITY, 0.0f, 0.0f};
+  add_vectors<T, H>(st, r[0]);
+  if (vectors > 32 * H) add_vectors<T, H>(st, r[1]);
+  if (single >= 0) add_value(st, edge);
+  const float mine = st.m;
+  int before = 0;
+  if (has && !(mine < given)) each([&](float v, int i) { before += lp_key(v, i) > given_key; });
+  // (the maximum of a lane of NaN alone is -inf: not under a given value of NaN or -inf)
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const Stat b{__shfl_xor_sync(0xFFFFFFFFu, st.m, o), __shfl_xor_sync(0xFFFFFFFFu, st.s, o), __shfl_xor_sync(0xFFFFFFFFu, st.t, o)};
+    st = lane & o ? join(b, st) : join(st, b);
+    before += __shfl_xor_sync(0xFFFFFFFFu, before, o);
+  }
+  const float base = st.m == -INFINITY ? 0.0f : st.m, lse = logf(st.s);
+  auto logprob = [&](float v) { return v == -INFINITY && !isnan(lse) ? -INFINITY : (v - base) - lse; };
+  if (lane == 0) {
+    a.logprobs[row] = has ? logprob(given) : id64 < 0 ? 0.0f : NAN;
+    a.ranks[row] = has ? before + 1 : 0;
+    a.entropy[row] = st.s == 0.0f ? 0.0f : lse - st.t * LN2 / st.s;
+  }
+  if (!a.top_n) return;
+  unsigned long long *cand = cand_all[warp], *best = best_all[warp];
+  int& found_at = found_all[warp];
+  if (lane == 0) found_at = 0;
+  best[lane] = 0;
+  int place = 0;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const float v = __shfl_sync(0xFFFFFFFFu, mine, j);
+    place += v > mine || (v == mine && j < lane);
+  }
+  const float limit = __shfl_sync(0xFFFFFFFFu, mine, __ffs(__ballot_sync(0xFFFFFFFFu, place == a.top_n - 1)) - 1);
+  __syncwarp();
+  if (mine >= limit)
+    each([&](float v, int i) {
+      if (v >= limit) {
+        const int slot = atomicAdd(&found_at, 1);
+        if (slot < LPW_ROOM) cand[slot] = lp_key(v, i);
+      }
+    });
+  __syncwarp();
+  const int found = found_at;
+  if (found <= LPW_ROOM && found >= min(a.top_n, a.vocab)) {
+    for (int i = lane; i < found; i += 32) {
+      const unsigned long long k = cand[i];
+      int at = 0;
+      for (int j = 0; j < found; ++j) at += cand[j] > k;
+      if (at < a.top_n) best[at] = k;
+    }
+  } else {                                        // many equal ones, or fewer numbers than alternatives: the next key of the row each time
+    unsigned long long last = ~0ull;
+    for (int n = 0; n < a.top_n && last; ++n) {
+      unsigned long long k = 0;
+      each([&](float v, int i) {
+        const unsigned long long q = lp_key(v, i);
+        if (q < last && q > k) k = q;
+      });
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const unsigned long long q = __shfl_xor_sync(0xFFFFFFFFu, k, o);
+        if (q > k) k = q;
+      }
+      if (lane == 0) best[n] = k;
+      last = k;
+    }
+  }
+  __syncwarp();
+  if (lane < a.top_n) {
+    const unsigned long long k = best[lane];
+    a.top_logprobs[row * a.top_n + lane] = k ? logprob(lp_key_value(k)) : -INFINITY;
+    a.top_ids[row * a.top_n + lane] = k ? 0x7FFFFFFF - (int)(uint32_t)k : -1;
+  }
+}
+
 template <typename T>
 static int launch_logprobs(const LogprobArgs& a, int64_t m, cudaStream_t st) {
+  if (a.vocab <= LPW_VECTORS * 32 * Vec<T>::N) {
+    logprobs_rows_kernel<T><<<(unsigned)((m + LPW_WARPS - 1) / LPW_WARPS), LPW_WARPS * 32, 0, st>>>(a, (int)m);
+    GSQ_CUDA_TRY(cudaGetLastError());
+    return GSQ_OK;
+  }
   DeviceInfo di;
   const int rc = device_info(&di);
   if (rc != GSQ_OK) return rc;
