@@ -376,7 +376,7 @@ int gsq_peer_reduce_error_flag(int* flag);
  *   the sum of the chosen ones where renormalize != 0) * scale. An expert with logit -inf or NaN is never chosen; a choice that
  *   finds none left is id -1, weight 0. Experts at +inf share the weight.
  * gsq_moe_layer: gsq_moe_route and gsq_moe_experts in one call, ids and weights kept in the workspace.
- * Limits: experts <= 1024, top_k <= 32, m <= 65536 (GSQ_ERR_TOO_LARGE).
+ * Limits: experts <= 1024, top_k <= 32, m <= 65536, hidden and inter <= 131072 (GSQ_ERR_TOO_LARGE).
  */
 #define GSQ_MOE_MAX_EXPERTS 1024
 #define GSQ_MOE_MAX_TOP_K 32

@@ -68,9 +68,21 @@ def _product(raw, t, q, unit):
     return mod.product_q81(_decode(raw, t), q.astype(np.int8), unit)
 
 
+def _parts(raw, t):
+    """Magnitude of the parts that a value's product is summed from: |value|, and where a block has minima the scaled quant and the
+    scaled minimum, which may cancel in the value but are added up apart."""
+    dec = _decode(raw, t)
+    if getattr(dec, "imin", None) is None:
+        return np.abs(values(raw, t))
+    n, k = dec.w8.shape
+    per = dec.imin.shape[1]
+    low = np.repeat(np.repeat(dec.dmin.astype(np.float64), per // dec.dmin.shape[1], 1) * dec.imin, k // per, 1)
+    return np.abs(values(raw, t) + low) + np.abs(low)
+
+
 def _magnitudes(raw, t, q, unit):
-    """Sum over the slices of the magnitudes that are added in fp32: no slice's term is larger than |w| . |x| over it."""
-    return (np.abs(q) * np.repeat(unit, 32, -1)) @ np.abs(values(raw, t)).T
+    """Sum of the magnitudes of what is added in fp32."""
+    return (np.abs(q) * np.repeat(unit, 32, -1)) @ _parts(raw, t).T
 
 
 def _sum_error(k):

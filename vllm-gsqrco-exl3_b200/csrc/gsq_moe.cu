@@ -1,5 +1,6 @@
-// Mixture-of-experts layer over GGUF-quantised experts for a few tokens (sm_100a): the router's choice, the 8-bit activations,
-// the host side. The products are in gsq_moe_dot.cu.
+// Mixture-of-experts layer over GGUF-quantised experts for a few tokens (sm_100a): the router's choice, the pairs of a token and
+// an expert gathered by expert, the weighted sum, the host side. The products are in gsq_moe_mma.cu (the four main types) and
+// gsq_moe_dot.cu (the others).
 //
 //   choice   s = softmax(logits) or sigmoid(logits); the top_k experts of largest logit (of largest s + bias where there is a
 //            bias), ties to the lowest number; weights s (/ their sum) * scale
@@ -180,6 +181,51 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(const MoeArgs a) {
   store_out_dyn(a.y, a.x_dtype, at + 3, s.w);
 }
 
+// Pairs by expert: group, list. One block. The order of an expert's pairs in the list is not the same every time, and no result
+// depends on it: a group's columns do not meet.
+constexpr int PLAN_THREADS = 1024;
+__global__ void __launch_bounds__(PLAN_THREADS) moe_plan_kernel(const MoeArgs a) {
+  __shared__ int count[GSQ_MOE_MAX_EXPERTS], place[GSQ_MOE_MAX_EXPERTS];
+  __shared__ int2 warp_sum[PLAN_THREADS / 32];
+  const int tid = threadIdx.x, lane = tid & 31, pairs = a.m * a.top_k;
+  count[tid] = 0;
+  __syncthreads();
+  for (int p = tid; p < pairs; p += PLAN_THREADS) {
+    const int e = moe_expert(a, p);
+    if (e >= 0) atomicAdd(&count[e], 1);
+  }
+  __syncthreads();
+  // places of the experts in the list and of their groups: sums over the experts before
+  const int n = count[tid], g = (n + 7) >> 3;
+  int2 upto = make_int2(n, g);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xFFFFFFFFu, upto.x, o), y = __shfl_up_sync(0xFFFFFFFFu, upto.y, o);
+    if (lane >= o) {
+      upto.x += x;
+      upto.y += y;
+    }
+  }
+  if (lane == 31) warp_sum[tid >> 5] = upto;
+  __syncthreads();
+  for (int w = 0; w < (tid >> 5); ++w) {
+    upto.x += warp_sum[w].x;
+    upto.y += warp_sum[w].y;
+  }
+  place[tid] = upto.x - n;
+  for (int i = 0; i < g; ++i) a.group[upto.y - g + i] = make_int4(tid, upto.x - n + 8 * i, min(8, n - 8 * i), 0);
+  if (tid == PLAN_THREADS - 1) *a.groups = upto.y;
+  __syncthreads();
+  for (int p = tid; p < pairs; p += PLAN_THREADS) {
+    const int e = moe_expert(a, p);
+    if (e >= 0) a.list[atomicAdd(&place[e], 1)] = p;
+  }
+}
+static_assert(PLAN_THREADS == GSQ_MOE_MAX_EXPERTS, "a thread an expert");
+
+// Tokens of one pass: the workspace holds that many, and the numbers of groups and tiles stay far from 2^31.
+constexpr int64_t PASS_TOKENS = 1024;
+
 // Workspace: pieces in the order of `next`, each 256-byte aligned.
 struct Pieces {
   size_t at = 0;
@@ -190,18 +236,22 @@ struct Pieces {
   }
 };
 struct MoeLayout {
-  size_t xq, xd, h, hq, hd, part, weights, ids, total;
+  size_t weights, ids, groups, group, list, xq, xd, h, hq, hd, part, total;
   MoeLayout(int64_t m, int64_t hidden, int64_t inter, int top_k) {
-    const size_t pairs = (size_t)m * top_k;
     Pieces p;
+    weights = p.next((size_t)m * top_k * 4);
+    ids = p.next((size_t)m * top_k * 4);
+    m = m < PASS_TOKENS ? m : PASS_TOKENS;
+    const size_t pairs = (size_t)m * top_k;
+    groups = p.next(4);
+    group = p.next(pairs * 16);
+    list = p.next(pairs * 4);
     xq = p.next((size_t)m * hidden);
     xd = p.next((size_t)m * hidden / 8);
     h = p.next(pairs * inter * 4);
     hq = p.next(pairs * inter);
     hd = p.next(pairs * inter / 8);
     part = p.next(pairs * hidden * 4);
-    weights = p.next(pairs * 4);
-    ids = p.next(pairs * 4);
     total = p.at;
   }
 };
@@ -228,7 +278,7 @@ static int check_moe(const gsq_moe* w, const void* x, int x_dtype, int64_t m, in
   if (m == 0) return GSQ_OK;
   if (!w->w13 || !w->w2 || !x || !y || (uintptr_t)w->w13 % 16 || (uintptr_t)w->w2 % 16) return GSQ_ERR_UNSUPPORTED;
   if (x_row_stride < 0 || (m > 1 && y_row_stride < w->hidden)) return GSQ_ERR_UNSUPPORTED;
-  if (w->hidden > (1 << 20) || w->inter > (1 << 20) || w->experts > GSQ_MOE_MAX_EXPERTS || top_k > GSQ_MOE_MAX_TOP_K || m > GSQ_MOE_MAX_TOKENS)
+  if (w->hidden > (1 << 17) || w->inter > (1 << 17) || w->experts > GSQ_MOE_MAX_EXPERTS || top_k > GSQ_MOE_MAX_TOP_K || m > GSQ_MOE_MAX_TOKENS)
     return GSQ_ERR_TOO_LARGE;
   if (!ws || ws_bytes < gsq_moe_workspace_bytes(m, w->hidden, w->inter, top_k) || (uintptr_t)ws % 256) return GSQ_ERR_SCRATCH;
   return GSQ_OK;
@@ -246,30 +296,51 @@ static int run_experts(const gsq_moe* w, const void* x, int x_dtype, int64_t m, 
   a.hidden = (int)w->hidden;
   a.inter = (int)w->inter;
   a.act = w->activation;
-  a.m = (int)m;
   a.top_k = top_k;
-  a.x = x;
   a.x_dtype = x_dtype;
   a.x_stride = x_row_stride;
-  a.x_vec = (uintptr_t)x % 16 == 0 && (m == 1 || x_row_stride * (x_dtype == GSQ_F32 ? 4 : 2) % 16 == 0);
-  a.weights = weights;
-  a.ids = ids;
+  const int64_t es = x_dtype == GSQ_F32 ? 4 : 2, id_bytes = ids64 ? 8 : 4;
+  a.x_vec = (uintptr_t)x % 16 == 0 && (m == 1 || x_row_stride * es % 16 == 0);
   a.ids64 = ids64;
-  a.y = y;
   a.y_stride = y_row_stride;
+  a.groups = (int*)(ws + l.groups);
+  a.group = (int4*)(ws + l.group);
+  a.list = (int*)(ws + l.list);
   a.xq = (int8_t*)(ws + l.xq);
   a.xd = (float*)(ws + l.xd);
   a.h = (float*)(ws + l.h);
   a.hq = (int8_t*)(ws + l.hq);
   a.hd = (float*)(ws + l.hd);
   a.part = (float*)(ws + l.part);
-  int rc = launch_quant(x, x_dtype, a.x_vec, x_row_stride, m, a.hidden, a.xq, a.xd, st);
-  if (rc == GSQ_OK) rc = moe_dot_gate_up(a, w->w13_type, st);
-  if (rc == GSQ_OK) rc = launch_quant(a.h, GSQ_F32, 1, a.inter, m * top_k, a.inter, a.hq, a.hd, st);
-  if (rc == GSQ_OK) rc = moe_dot_down(a, w->w2_type, st);
-  if (rc != GSQ_OK) return rc;
-  moe_combine_kernel<<<(unsigned)((m * (a.hidden >> 2) + 255) / 256), 256, 0, st>>>(a);
-  GSQ_CUDA_TRY(cudaGetLastError());
+  const bool up_mma = moe_mma_serves(w->w13_type, a.hidden), down_mma = moe_mma_serves(w->w2_type, a.inter);
+  for (int64_t t0 = 0; t0 < m; t0 += PASS_TOKENS) {
+    a.m = (int)(m - t0 < PASS_TOKENS ? m - t0 : PASS_TOKENS);
+    a.x = (const uint8_t*)x + t0 * x_row_stride * es;
+    a.y = (uint8_t*)y + t0 * y_row_stride * es;
+    a.weights = weights + t0 * top_k;
+    a.ids = (const uint8_t*)ids + t0 * top_k * id_bytes;
+    int rc = GSQ_OK;
+    if (up_mma || down_mma) {
+      moe_plan_kernel<<<1, PLAN_THREADS, 0, st>>>(a);
+      GSQ_CUDA_TRY(cudaGetLastError());
+    }
+    if (up_mma) {
+      rc = moe_mma_product(a, w->w13_type, false, st);
+    } else {
+      rc = launch_quant(a.x, x_dtype, a.x_vec, x_row_stride, a.m, a.hidden, a.xq, a.xd, st);
+      if (rc == GSQ_OK) rc = moe_dot_gate_up(a, w->w13_type, st);
+    }
+    if (rc != GSQ_OK) return rc;
+    if (down_mma) {
+      rc = moe_mma_product(a, w->w2_type, true, st);
+    } else {
+      rc = launch_quant(a.h, GSQ_F32, 1, a.inter, (int64_t)a.m * top_k, a.inter, a.hq, a.hd, st);
+      if (rc == GSQ_OK) rc = moe_dot_down(a, w->w2_type, st);
+    }
+    if (rc != GSQ_OK) return rc;
+    moe_combine_kernel<<<(unsigned)(((int64_t)a.m * (a.hidden >> 2) + 255) / 256), 256, 0, st>>>(a);
+    GSQ_CUDA_TRY(cudaGetLastError());
+  }
   return GSQ_OK;
 }
 

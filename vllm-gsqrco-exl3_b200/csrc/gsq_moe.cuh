@@ -25,6 +25,10 @@ struct MoeArgs {
   float *xd, *hd;              // their scales, one per 32 values
   float* h;                    // [pairs][inter]: act(gate) * up
   float* part;                 // [pairs][hidden]: weight times down product
+  // pairs by expert, at most 8 to a group
+  int* groups;                 // how many
+  int4* group;                 // expert, first place in the list, pairs
+  int* list;                   // pairs
 };
 
 // Expert of a pair, -1 for one that is not here (negative or past the last).
@@ -63,5 +67,8 @@ __device__ __forceinline__ float moe_act(int act, float g) {
 // gsq_moe_dot.cu: the two products for every pair, from xq / xd to h, from hq / hd to part
 int moe_dot_gate_up(const MoeArgs& a, int type, cudaStream_t st);
 int moe_dot_down(const MoeArgs& a, int type, cudaStream_t st);
+// gsq_moe_mma.cu: the same by groups, from x to h, from h to part
+bool moe_mma_serves(int type, int k);
+int moe_mma_product(const MoeArgs& a, int type, bool down, cudaStream_t st);
 
 }  // namespace gsq
