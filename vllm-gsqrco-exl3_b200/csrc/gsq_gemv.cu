@@ -1176,18 +1176,16 @@ extern "C" int gsq_debug_force_cluster_size(int cs) {
 namespace gsq {
 int gemm_error_flag(int* flag);  // gsq_gemm.cu
 int mmv_error_flags(int* peer, int* copy);  // gsq_mmv.cu
-int moe_error_flag(int* flag);  // gsq_moe_mma.cu
 }
 
 extern "C" int gsq_device_error_flag(int* flag) {
   if (!flag) return GSQ_ERR_UNSUPPORTED;
-  int a = 0, b = 0, c = 0, d = 0, peer = 0;
+  int a = 0, b = 0, c = 0, peer = 0;
   GSQ_CUDA_TRY(cudaMemcpyFromSymbol(&a, gsq::g_gemv_error, sizeof(int)));
   int rc = gsq::gemm_error_flag(&b);
   if (rc == GSQ_OK) rc = gsq::mmv_error_flags(&peer, &c);
-  if (rc == GSQ_OK) rc = gsq::moe_error_flag(&d);
   if (rc != GSQ_OK) return rc;
-  *flag = a | b | c | d;
+  *flag = a | b | c;
   return GSQ_OK;
 }
 

@@ -181,12 +181,13 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(const MoeArgs a) {
   store_out_dyn(a.y, a.x_dtype, at + 3, s.w);
 }
 
-// Pairs by expert: group, list. One block. The order of an expert's pairs in the list is not the same every time, and no result
-// depends on it: a group's columns do not meet.
+// Pairs by expert: group, list. One block. An expert's pairs stay in their order, so that the same ones share a group every time (a
+// group's size decides the order of its sums).
 constexpr int PLAN_THREADS = 1024;
 __global__ void __launch_bounds__(PLAN_THREADS) moe_plan_kernel(const MoeArgs a) {
   __shared__ int count[GSQ_MOE_MAX_EXPERTS], place[GSQ_MOE_MAX_EXPERTS];
   __shared__ int2 warp_sum[PLAN_THREADS / 32];
+  __shared__ uint8_t of_warp[PLAN_THREADS / 32][GSQ_MOE_MAX_EXPERTS];   // pairs of an expert among a warp's 32
   const int tid = threadIdx.x, lane = tid & 31, pairs = a.m * a.top_k;
   count[tid] = 0;
   __syncthreads();
@@ -215,10 +216,23 @@ __global__ void __launch_bounds__(PLAN_THREADS) moe_plan_kernel(const MoeArgs a)
   place[tid] = upto.x - n;
   for (int i = 0; i < g; ++i) a.group[upto.y - g + i] = make_int4(tid, upto.x - n + 8 * i, min(8, n - 8 * i), 0);
   if (tid == PLAN_THREADS - 1) *a.groups = upto.y;
-  __syncthreads();
-  for (int p = tid; p < pairs; p += PLAN_THREADS) {
-    const int e = moe_expert(a, p);
-    if (e >= 0) a.list[atomicAdd(&place[e], 1)] = p;
+  const int warp = tid >> 5;
+  for (int p0 = 0; p0 < pairs; p0 += PLAN_THREADS) {
+    const int p = p0 + tid, e = p < pairs ? moe_expert(a, p) : -1;
+    for (int i = lane; i < a.experts; i += 32) of_warp[warp][i] = 0;
+    __syncwarp();
+    const uint32_t same = __match_any_sync(0xFFFFFFFFu, e);
+    if (e >= 0 && lane == __ffs(same) - 1) of_warp[warp][e] = (uint8_t)__popc(same);
+    __syncthreads();
+    if (e >= 0) {
+      int at = place[e] + __popc(same & ((1u << lane) - 1));
+      for (int w = 0; w < warp; ++w) at += of_warp[w][e];
+      a.list[at] = p;
+    }
+    __syncthreads();
+    if (tid < a.experts)
+      for (int w = 0; w < PLAN_THREADS / 32; ++w) place[tid] += of_warp[w][tid];
+    __syncthreads();
   }
 }
 static_assert(PLAN_THREADS == GSQ_MOE_MAX_EXPERTS, "a thread an expert");

@@ -3,18 +3,29 @@
 // The pairs of a token and one of its experts are gathered by expert, at most 8 to a group (gsq_moe.cu), so that an expert's
 // weights are read and decoded once for 8 tokens. A tile is 16 weight rows: 8 gate and the 8 up rows of the same channels, which
 // leaves a channel's gate and up sums in one lane, or 16 rows of the down weights. The list of (group, tile) is cut into one
-// contiguous range a block, one block an SM.
+// contiguous range a block, one block an SM; a block takes as many groups of its range at a time as its columns of
+// activations hold (a batch, mostly all of them), and cuts the batch's superblocks into 16 equal contiguous chunks, one a warp.
 //
-//   * Weights: each warp has a ring of bulk copies of its own (16 rows x 1 or 2 superblocks a stage, one copy a row), filled ahead over
-//     tiles and groups, so the stream does not stop where a group ends. Rows of 210- and 110-byte blocks start at any even address:
-//     a copy begins at the 16-byte boundary before, and the rows are read at their offset.
-//   * Activations: the block takes its group's rows (X, or the activated products), quantises them into shared memory in the order of
-//     the tensor-core instruction's B fragment. Columns past the group's are left as they are: they only reach results that are not stored.
+//   * Weights: each warp has a ring of asynchronous copies of its own (16 rows x 1 superblock a stage, consecutive lanes on consecutive
+//     16-byte pieces of a row), filled ahead over tiles and batches, so the stream does not stop. Rows of 210- and 110-byte blocks start at any even address: copies begin at
+//     the 16-byte boundary before, and the rows are read at their offset. (One bulk copy a row was a loop over the 16 lanes that
+//     issue them: 95 of 427 instructions a superblock.)
+//   * Activations: the block takes its batch's rows (X, or the activated products), quantises them into shared memory in the order of
+//     the tensor-core instruction's B fragment. An instruction takes the 8 columns from its group's first on; what it finds past the
+//     group's own only reaches sums that are not stored.
 //   * Product: mma.sync m16n8k32 on bytes (m16n8k16 for Q6_K, whose sub-scales cover 16 values); a lane decodes exactly its share of
-//     the A fragment. Sums leave the instruction on the bit pattern of 1.5 * 2^23, so fma(sum, dA, -1.5 * 2^23 dA) is the exact integer
-//     times d * sub-scale without a conversion; the second fma scales by the activations. Q4_K's minima are a product of their
-//     own, min [16 rows x 8 slices] times d_x * sum of the quants [8 slices x 8 columns], in three tf32 parts that hold all 24 bits.
-//   * Few tiles a block: 2 to 16 warps share a tile along K and add their sums through shared memory in a fixed order.
+//     the A fragment. Every sub-scale's sum has to be scaled on its own, and that, not the instruction, is the cost: with a column for
+//     each of 8 tokens it is 14 instructions a slice and lane. A group of 1, 2 or 4 tokens therefore gives the free columns to other
+//     slices: the instruction of slice j has the activations in the columns of slice j and zeros in the others, and the sums of 8, 4
+//     or 2 slices come out side by side in one C fragment, scaled at once. (Q4_K, instructions a superblock of 16 rows: 357 with one
+//     form for all, of which DRAM's rate leaves room for 250.)
+//   * Sums leave the instruction on the bit pattern of 1.5 * 2^23, so fma(sum, dA, -1.5 * 2^23 dA) is the exact integer times
+//     d * sub-scale without a conversion; the second fma scales by the activations. Q4_K's high nibbles are multiplied where they
+//     are, as unsigned bytes 16 times their value. Its minima, for 4 and 8 tokens, are a product of their own, min [16 rows x 8
+//     slices] times d_x * sum of the quants [8 slices x 8 columns], in three tf32 parts that hold all 24 bits.
+//   * A tile that several warps have parts of is added up by the warp that has its beginning, in the order of the warps.
+#include <type_traits>
+
 #include "gsq_moe.cuh"
 #include "gsq_tables.h"
 
@@ -28,56 +39,45 @@ constexpr float MAGIC_F = 12582912.0f;
 
 __device__ const uint32_t g_iq3s[512] = GSQ_IQ3S_GRID_INIT;
 __constant__ __align__(16) int8_t c_iq4[16] = GSQ_IQ4NL_VALUES_INIT;
-__device__ int g_error = 0;                  // sticky: a wait on a copy gave up (gsq_device_error_flag)
 
 __host__ __device__ constexpr int bs(int kind) { return kind == Q4K ? 144 : kind == Q6K ? 210 : kind == IQ3S ? 110 : 136; }
-// Bytes between the rows of a stage: what a copy may take (14 bytes in front, the size to a multiple of 16), with 8 rows' 32 bytes on
-// different banks where the row's own length does not do it.
-__host__ __device__ constexpr int pitch(int kind, int sbs) {
-  return kind == Q4K ? (sbs == 2 ? 288 : 160) : kind == Q6K ? (sbs == 2 ? 480 : 224) : kind == IQ3S ? (sbs == 2 ? 240 : 160) : (sbs == 2 ? 288 : 160);
-}
+// Bytes between the rows of a stage: what a row's pieces may take (up to 14 bytes in front, 16-byte pieces), at distances that put what a
+// warp reads at once on different banks.
+__host__ __device__ constexpr int pitch(int kind) { return kind == Q4K ? 160 : kind == Q6K ? 240 : 144; }
 constexpr int GRID_COPIES = 8;               // of IQ3_S's codebook in shared memory, one for lanes l, l + 8, ...
-__host__ __device__ constexpr size_t fixed_smem(int kind, int k) {   // all but the ring
-  return (size_t)k * 8 + (size_t)k / 32 * 32 + (kind == Q4K ? (size_t)k / 256 * 768 : 0) + (kind == IQ3S ? 512 * 4 * GRID_COPIES : 0) + 2 * WARPS * 512;
+constexpr int WINDOW = 64;                   // groups of a block that are looked up at a time
+__host__ __device__ constexpr size_t fixed_smem(int kind, int k, int cap) {   // all but the ring
+  return (size_t)k * cap + (size_t)k / 32 * cap * 4 + (kind == Q4K ? (size_t)k / 256 * cap * 128 : 0) + (kind == IQ3S ? 512 * 4 * GRID_COPIES : 0) +
+         2 * WARPS * 512;
 }
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void bar_init(uint32_t bar) { asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void copy_row(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
+__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the calling thread's last n groups of copies are done.
+template <int N>
+__device__ __forceinline__ void wait_all_but() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-// Gives up after about a second and raises the flag: the sums are then wrong, and nothing waits for ever.
-__device__ __forceinline__ void bar_wait(uint32_t bar, uint32_t parity) {
-  uint32_t done = 0;
-  for (int spin = 0; spin < (1 << 22); ++spin) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-        "selp.u32 %0, 1, 0, p;\n"
-        "}\n"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (done) return;
-  }
-  atomicExch(&g_error, 1);
-}
-__device__ __forceinline__ void warps_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
-__device__ __forceinline__ void mma_k32(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b, int init) {
-  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-      : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y), "r"(init));
+// C += A B, signed bytes (UA: A unsigned)
+template <bool UA>
+__device__ __forceinline__ void mma_k32(int (&c)[4], const uint32_t (&a)[4], uint2 b) {
+  if constexpr (UA)
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
+  else
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
 }
 __device__ __forceinline__ void mma_k16(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t b) {
-  asm("mma.sync.aligned.m16n8k16.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%7, %7, %7, %7};"
-      : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-      : "r"(a0), "r"(a1), "r"(b), "r"(0));
+  asm("mma.sync.aligned.m16n8k16.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%0, %1, %2, %3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(b));
 }
 __device__ __forceinline__ void mma_tf32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, float2 b) {
   asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -93,142 +93,243 @@ __device__ __forceinline__ uint32_t lds16(const uint8_t* p) { return *reinterpre
 __device__ __forceinline__ uint32_t lds32(const uint8_t* p) { return *reinterpret_cast<const uint32_t*>(p); }
 __device__ __forceinline__ uint32_t lds32h(const uint8_t* p) { return prmt(lds16(p), lds16(p + 2), 0x5410); }   // from an even address
 
-// What a lane (g = lane / 4, t = lane % 4) reads of the staged activations of one superblock.
-struct Act {
-  const uint8_t* q;        // [slice][column][32 bytes], at this lane's 8 bytes of column g
-  const float* d;          // [slice][column], at columns 2 t, 2 t + 1
-  const float* mins;       // [part][t][column][2], at this lane's pair
+// How a group of up to TT tokens uses the 8 columns of a C fragment: NJ parts (slices of 32 values; of 16 for Q6_K) times TT tokens,
+// column j TT + token. A superblock is NC fragments. Lane (g, t) feeds column g, and has the sums of columns 2 t, 2 t + 1.
+template <int KIND, int TT>
+struct Columns {
+  static constexpr int NJ = 8 / TT, PARTS = KIND == Q6K ? 16 : 8, NC = PARTS / NJ;
+  static __device__ __forceinline__ int fed_part(int g) { return g / TT; }
+  static __device__ __forceinline__ int fed_token(int g) { return g % TT; }
+  static __device__ __forceinline__ int part(int t, int c) { return (2 * t + c) / TT; }   // (c: 0 or 1; the same for both unless TT is 1)
 };
-__device__ __forceinline__ uint2 act_q(const Act& x, int s) { return *reinterpret_cast<const uint2*>(x.q + 256 * s); }
-__device__ __forceinline__ float2 act_d(const Act& x, int s) { return *reinterpret_cast<const float2*>(x.d + 8 * s); }
 
-// acc += (row scale) * (activation scale) * sum, for the four sums of a lane (rows g, g + 8; columns 2 t, 2 t + 1), sums on MAGIC.
-__device__ __forceinline__ void scale_sums(float (&acc)[4], const int (&c)[4], float a0, float a1, float2 d) {
-  const float m0 = -MAGIC_F * a0, m1 = -MAGIC_F * a1;
-  acc[0] = fmaf(fmaf(__int_as_float(c[0]), a0, m0), d.x, acc[0]);
-  acc[1] = fmaf(fmaf(__int_as_float(c[1]), a0, m0), d.y, acc[1]);
-  acc[2] = fmaf(fmaf(__int_as_float(c[2]), a1, m1), d.x, acc[2]);
-  acc[3] = fmaf(fmaf(__int_as_float(c[3]), a1, m1), d.y, acc[3]);
+// What a lane reads of the staged activations of one superblock, CAP columns a slice.
+template <int KIND, int CAP, int TT>
+struct Act {
+  using Col = Columns<KIND, TT>;
+  const uint8_t* q;        // [slice][column][32 bytes]
+  const float* d;          // [slice][column]
+  const float* sums;       // [slice][column]: d * sum of the quants (Q4_K)
+  const float* mins;       // the same in parts, [part][column][t][2]
+  // col: the group's first column
+  __device__ __forceinline__ Act(const uint8_t* q_s, const float* d_s, const float* min_s, int nsb, int sb, int col, int g, int t) {
+    const int j = Col::fed_part(g), i = Col::part(t, 0), s = KIND == Q6K ? i >> 1 : i;
+    q = q_s + ((sb * 8 + (KIND == Q6K ? j >> 1 : j)) * CAP + col + Col::fed_token(g)) * 32 + 8 * t + (KIND == Q6K ? 4 * (j & 1) : 0);
+    d = d_s + (sb * 8 + s) * CAP + col + 2 * t % TT;
+    sums = min_s + (sb * 8 + s) * CAP + col + 2 * t % TT;
+    mins = min_s + nsb * 8 * CAP + sb * (CAP * 24) + ((col + g) * 4 + t) * 2;
+  }
+  __device__ __forceinline__ void next() {
+    q += CAP * 256;
+    d += CAP * 8;
+    sums += CAP * 8;
+    mins += CAP * 24;
+  }
+  // this lane's words of the part that it feeds in fragment c
+  __device__ __forceinline__ uint2 quants(int c) const { return *reinterpret_cast<const uint2*>(q + CAP * 32 * Col::NJ * c); }
+  __device__ __forceinline__ uint32_t quants16(int c) const {
+    return *reinterpret_cast<const uint32_t*>(q + (TT == 8 ? CAP * 32 * (c >> 1) + 4 * (c & 1) : CAP * 16 * Col::NJ * c));
+  }
+  static __device__ __forceinline__ float2 two(const float* p, int c) {
+    const int s = KIND != Q6K ? Col::NJ * c : TT == 8 ? c >> 1 : Col::NJ / 2 * c;
+    if constexpr (TT > 1) return *reinterpret_cast<const float2*>(p + CAP * s);
+    return make_float2(p[CAP * s], p[CAP * (s + (KIND != Q6K))]);   // (Q6_K: two halves of a slice)
+  }
+  __device__ __forceinline__ float2 scales(int c) const { return two(d, c); }
+  __device__ __forceinline__ float2 quant_sums(int c) const { return two(sums, c); }
+  __device__ __forceinline__ float2 minima(int part) const { return *reinterpret_cast<const float2*>(mins + CAP * 8 * part); }
+};
+
+// Byte `at` (of 8 in two words) as a number on 2^23.
+__device__ __forceinline__ float byte_on_2_23(const uint32_t (&w)[2], bool upper, uint32_t at) {
+  return __uint_as_float(prmt(upper ? w[1] : w[0], 0x4B000000u, 0x7440u | at));
 }
 
-// One superblock of 16 rows: b0, b1 = the blocks of rows g and g + 8.
-template <int KIND>
-__device__ __forceinline__ void superblock(const uint8_t* b0, const uint8_t* b1, const Act& x, int t, const uint32_t* grid, float (&acc)[4]) {
+// One superblock of 16 rows: b0, b1 = the blocks of rows g and g + 8; acc: rows g, g + 8 by columns 2 t, 2 t + 1 of the C fragments.
+template <int KIND, int CAP, int TT>
+__device__ __forceinline__ void superblock(const uint8_t* b0, const uint8_t* b1, const Act<KIND, CAP, TT>& x, int g, int t, const uint32_t* grid,
+                                           float (&acc)[4]) {
+  using Col = Columns<KIND, TT>;
+  constexpr int NJ = Col::NJ, NC = Col::NC;
+  const int fed = Col::fed_part(g), part0 = Col::part(t, 0), part1 = Col::part(t, 1);   // (parts within a fragment)
+  // what the rows' scales come from
+  uint32_t sc[2][2], mn[2][2];
+  uint2 h0, h1;
+  float d0, d1;
   if constexpr (KIND == Q4K) {
-    const uint4 h0 = *reinterpret_cast<const uint4*>(b0), h1 = *reinterpret_cast<const uint4*>(b1);
-    const uint32_t sc[2][2] = {{h0.y & 0x3F3F3F3Fu, (h0.w & 0x0F0F0F0Fu) | ((h0.y >> 2) & 0x30303030u)},
-                               {h1.y & 0x3F3F3F3Fu, (h1.w & 0x0F0F0F0Fu) | ((h1.y >> 2) & 0x30303030u)}};
-    const uint32_t mn[2][2] = {{h0.z & 0x3F3F3F3Fu, ((h0.w >> 4) & 0x0F0F0F0Fu) | ((h0.z >> 2) & 0x30303030u)},
-                               {h1.z & 0x3F3F3F3Fu, ((h1.w >> 4) & 0x0F0F0F0Fu) | ((h1.z >> 2) & 0x30303030u)}};
-    const float d0 = h2f(h0.x), d1 = h2f(h1.x), n0 = -8388608.0f * d0, n1 = -8388608.0f * d1;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint2 q0 = *reinterpret_cast<const uint2*>(b0 + 16 + 32 * j + 8 * t), q1 = *reinterpret_cast<const uint2*>(b1 + 16 + 32 * j + 8 * t);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int s = 2 * j + h;
-        int c[4];
-        mma_k32(c, (q0.x >> (4 * h)) & 0x0F0F0F0Fu, (q1.x >> (4 * h)) & 0x0F0F0F0Fu, (q0.y >> (4 * h)) & 0x0F0F0F0Fu,
-                (q1.y >> (4 * h)) & 0x0F0F0F0Fu, act_q(x, s), MAGIC);
-        // the sub-scale as the low byte of 2^23's bits, times d, less 2^23 d: exact
-        const float a0 = fmaf(__uint_as_float(prmt(sc[0][s >> 2], 0x4B000000u, 0x7440 | (s & 3))), d0, n0);
-        const float a1 = fmaf(__uint_as_float(prmt(sc[1][s >> 2], 0x4B000000u, 0x7440 | (s & 3))), d1, n1);
-        scale_sums(acc, c, a0, a1, act_d(x, s));
-      }
-    }
-    // minima: rows g, g + 8 by slices t, t + 4
-    auto min_of = [&](uint32_t w) { return __float_as_uint(__uint_as_float(prmt(w, 0x4B000000u, 0x7440 | t)) - 8388608.0f); };
-    const uint32_t m0 = min_of(mn[0][0]), m1 = min_of(mn[1][0]), m2 = min_of(mn[0][1]), m3 = min_of(mn[1][1]);
-    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int p = 2; p >= 0; --p) mma_tf32(c, m0, m1, m2, m3, *reinterpret_cast<const float2*>(x.mins + 64 * p));
-    const float e0 = -h2f(h0.x >> 16), e1 = -h2f(h1.x >> 16);
-    acc[0] = fmaf(e0, c[0], acc[0]);
-    acc[1] = fmaf(e0, c[1], acc[1]);
-    acc[2] = fmaf(e1, c[2], acc[2]);
-    acc[3] = fmaf(e1, c[3], acc[3]);
+    const uint4 r0 = *reinterpret_cast<const uint4*>(b0), r1 = *reinterpret_cast<const uint4*>(b1);
+    sc[0][0] = r0.y & 0x3F3F3F3Fu;
+    sc[0][1] = (r0.w & 0x0F0F0F0Fu) | ((r0.y >> 2) & 0x30303030u);
+    sc[1][0] = r1.y & 0x3F3F3F3Fu;
+    sc[1][1] = (r1.w & 0x0F0F0F0Fu) | ((r1.y >> 2) & 0x30303030u);
+    mn[0][0] = r0.z & 0x3F3F3F3Fu;
+    mn[0][1] = ((r0.w >> 4) & 0x0F0F0F0Fu) | ((r0.z >> 2) & 0x30303030u);
+    mn[1][0] = r1.z & 0x3F3F3F3Fu;
+    mn[1][1] = ((r1.w >> 4) & 0x0F0F0F0Fu) | ((r1.z >> 2) & 0x30303030u);
+    h0.x = r0.x;
+    h1.x = r1.x;
+    d0 = h2f(r0.x);
+    d1 = h2f(r1.x);
   } else if constexpr (KIND == IQ4XS) {
-    const uint2 h0 = *reinterpret_cast<const uint2*>(b0), h1 = *reinterpret_cast<const uint2*>(b1);
-    const float d0 = h2f(h0.x), d1 = h2f(h1.x);
-    const uint32_t t0 = reinterpret_cast<const uint32_t*>(c_iq4)[0], t1 = reinterpret_cast<const uint32_t*>(c_iq4)[1],
-                   t2 = reinterpret_cast<const uint32_t*>(c_iq4)[2], t3 = reinterpret_cast<const uint32_t*>(c_iq4)[3];
-    // 8 indices -> two words of values in the order of the nibbles: value 4 t, 16 + 4 t, 4 t + 1, ... (the activations have that order)
-    auto look_up = [&](uint32_t v, uint32_t& lo, uint32_t& hi) {
-      const uint32_t s = v & 0x77777777u, pick = ((v >> 1) & 0x44444444u) | 0x32103210u;
-      lo = prmt(prmt(t0, t1, s), prmt(t2, t3, s), pick);
-      hi = prmt(prmt(t0, t1, s >> 16), prmt(t2, t3, s >> 16), pick >> 16);
-    };
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      uint32_t a0, a1, a2, a3;
-      look_up(lds32(b0 + 8 + 16 * s + 4 * t), a0, a2);
-      look_up(lds32(b1 + 8 + 16 * s + 4 * t), a1, a3);
-      int c[4];
-      mma_k32(c, a0, a1, a2, a3, act_q(x, s), MAGIC);
-      const int l0 = (int)(((h0.y >> (4 * s)) & 15u) | (((h0.x >> (16 + 2 * s)) & 3u) << 4));
-      const int l1 = (int)(((h1.y >> (4 * s)) & 15u) | (((h1.x >> (16 + 2 * s)) & 3u) << 4));
-      scale_sums(acc, c, d0 * (__int_as_float(MAGIC + l0) - (MAGIC_F + 32.0f)), d1 * (__int_as_float(MAGIC + l1) - (MAGIC_F + 32.0f)), act_d(x, s));
-    }
+    h0 = *reinterpret_cast<const uint2*>(b0);
+    h1 = *reinterpret_cast<const uint2*>(b1);
+    d0 = h2f(h0.x);
+    d1 = h2f(h1.x);
   } else if constexpr (KIND == IQ3S) {
-    const float d0 = h2f(lds16(b0)), d1 = h2f(lds16(b1));
-    const uint32_t ls0 = lds32h(b0 + 106), ls1 = lds32h(b1 + 106);
-    auto value = [&](uint32_t low, uint32_t high, uint32_t signs) {   // index low | high << 8, negated where a sign bit is set
-      const uint32_t v = grid[(low | (high << 8)) * GRID_COPIES];
-      const uint32_t ones = ((signs & 15u) * 0x00204081u) & 0x01010101u;
-      return (v ^ (ones * 255u)) + ones;
-    };
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      const uint32_t q0 = lds16(b0 + 2 + 8 * s + 2 * t), q1 = lds16(b1 + 2 + 8 * s + 2 * t);
-      const uint32_t h0 = b0[66 + s] >> (2 * t), h1 = b1[66 + s] >> (2 * t), g0 = b0[74 + 4 * s + t], g1 = b1[74 + 4 * s + t];
-      int c[4];
-      mma_k32(c, value(q0 & 255u, h0 & 1u, g0), value(q1 & 255u, h1 & 1u, g1), value(q0 >> 8, (h0 >> 1) & 1u, g0 >> 4),
-              value(q1 >> 8, (h1 >> 1) & 1u, g1 >> 4), act_q(x, s), MAGIC);
-      const int l0 = 1 + 2 * (int)((ls0 >> (4 * s)) & 15u), l1 = 1 + 2 * (int)((ls1 >> (4 * s)) & 15u);
-      scale_sums(acc, c, d0 * (__int_as_float(MAGIC + l0) - MAGIC_F), d1 * (__int_as_float(MAGIC + l1) - MAGIC_F), act_d(x, s));
-    }
+    h0.x = lds32h(b0 + 106);
+    h1.x = lds32h(b1 + 106);
+    d0 = h2f(lds16(b0));
+    d1 = h2f(lds16(b1));
   } else {
-    // value q - 32 (q six bits) as q << 2 with the top bit flipped: four times it, as a signed byte
-    const float d0 = 0.25f * h2f(lds16(b0 + 208)), d1 = 0.25f * h2f(lds16(b1 + 208));
-    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    d0 = 0.25f * h2f(lds16(b0 + 208));
+    d1 = 0.25f * h2f(lds16(b1 + 208));
+  }
+  // d * sub-scale of row 0 / 1 (of this lane's two) for column c (0 / 1) of fragment f: exact
+  auto row_scale = [&](int row, int f, int c) {
+    const int p = c ? part1 : part0;
+    const float d = row ? d1 : d0;
+    if constexpr (KIND == Q4K) {
+      // (the parity of the slice says which nibble: odd ones are 16 times too large)
+      const bool upper = TT == 1 ? p >= 4 : TT == 2 ? f : TT == 4 ? f >> 1 : f >> 2;
+      const uint32_t at = TT == 1 ? p & 3 : TT == 2 ? p : TT == 4 ? (f & 1) * 2 + p : f & 3;
+      const bool odd = TT == 8 ? f & 1 : TT == 1 ? c : p & 1;
+      const float e = odd ? 0.0625f * d : d;
+      return fmaf(byte_on_2_23(sc[row], upper, at), e, -8388608.0f * e);
+    } else if constexpr (KIND == IQ4XS) {
+      const uint2 h = row ? h1 : h0;
+      const int s = f * NJ + p, l = (int)(((h.y >> (4 * s)) & 15u) | (((h.x >> (16 + 2 * s)) & 3u) << 4));
+      return d * (__int_as_float(MAGIC + l) - (MAGIC_F + 32.0f));
+    } else if constexpr (KIND == IQ3S) {
+      const int s = f * NJ + p, l = 1 + 2 * (int)(((row ? h1.x : h0.x) >> (4 * s)) & 15u);
+      return d * (__int_as_float(MAGIC + l) - MAGIC_F);
+    } else {
+      const int l = *reinterpret_cast<const int8_t*>((row ? b1 : b0) + 192 + f * NJ + p);
+      return d * (__int_as_float(MAGIC + l) - MAGIC_F);
+    }
+  };
+  // raw words that several slices share
+  uint2 q4[2];
+  uint32_t l6[2][2][2], h6[2][2];
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      uint32_t h[2][2], l[2][2][2];   // [row][half of 16 bytes], ql: [row][64-value half][half of 16 bytes]
+  for (int f = 0; f < NC; ++f) {
+    int c[4] = {MAGIC, MAGIC, MAGIC, MAGIC};
+    uint2 fed_words = make_uint2(0, 0);
+    if constexpr (KIND == Q6K) fed_words.x = x.quants16(f);
+    else fed_words = x.quants(f);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        h[0][e] = lds32h(b0 + 128 + 32 * n + 16 * e + 4 * t);
-        h[1][e] = lds32h(b1 + 128 + 32 * n + 16 * e + 4 * t);
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          l[0][r][e] = lds32h(b0 + 64 * n + 32 * r + 16 * e + 4 * t);
-          l[1][r][e] = lds32h(b1 + 64 * n + 32 * r + 16 * e + 4 * t);
+    for (int j = 0; j < NJ; ++j) {
+      const int s = f * NJ + j;        // part of the superblock
+      uint2 b = fed_words;
+      if (TT < 8 && fed != j) b = make_uint2(0, 0);
+      uint32_t a[4];
+      if constexpr (KIND == Q4K) {
+        if ((s & 1) == 0) {
+          q4[0] = *reinterpret_cast<const uint2*>(b0 + 16 + 16 * s + 8 * t);
+          q4[1] = *reinterpret_cast<const uint2*>(b1 + 16 + 16 * s + 8 * t);
         }
-      }
+        const uint32_t m = s & 1 ? 0xF0F0F0F0u : 0x0F0F0F0Fu;
+        a[0] = q4[0].x & m;
+        a[1] = q4[1].x & m;
+        a[2] = q4[0].y & m;
+        a[3] = q4[1].y & m;
+        mma_k32<true>(c, a, b);
+      } else if constexpr (KIND == IQ4XS) {
+        const uint32_t t0 = reinterpret_cast<const uint32_t*>(c_iq4)[0], t1 = reinterpret_cast<const uint32_t*>(c_iq4)[1],
+                       t2 = reinterpret_cast<const uint32_t*>(c_iq4)[2], t3 = reinterpret_cast<const uint32_t*>(c_iq4)[3];
+        // 8 indices -> two words of values in the order of the nibbles: value 4 t, 16 + 4 t, 4 t + 1, ... (the activations have that order)
+        auto look_up = [&](uint32_t v, uint32_t& lo, uint32_t& hi) {
+          const uint32_t i = v & 0x77777777u, pick = ((v >> 1) & 0x44444444u) | 0x32103210u;
+          lo = prmt(prmt(t0, t1, i), prmt(t2, t3, i), pick);
+          hi = prmt(prmt(t0, t1, i >> 16), prmt(t2, t3, i >> 16), pick >> 16);
+        };
+        look_up(lds32(b0 + 8 + 16 * s + 4 * t), a[0], a[2]);
+        look_up(lds32(b1 + 8 + 16 * s + 4 * t), a[1], a[3]);
+        mma_k32<false>(c, a, b);
+      } else if constexpr (KIND == IQ3S) {
+        auto value = [&](uint32_t low, uint32_t high, uint32_t signs) {   // index low | high << 8, negated where a sign bit is set
+          const uint32_t v = grid[(low | (high << 8)) * GRID_COPIES];
+          const uint32_t ones = ((signs & 15u) * 0x00204081u) & 0x01010101u;
+          return (v ^ (ones * 255u)) + ones;
+        };
+        const uint32_t q0 = lds16(b0 + 2 + 8 * s + 2 * t), q1 = lds16(b1 + 2 + 8 * s + 2 * t);
+        const uint32_t e0 = b0[66 + s] >> (2 * t), e1 = b1[66 + s] >> (2 * t), g0 = b0[74 + 4 * s + t], g1 = b1[74 + 4 * s + t];
+        a[0] = value(q0 & 255u, e0 & 1u, g0);
+        a[1] = value(q1 & 255u, e1 & 1u, g1);
+        a[2] = value(q0 >> 8, (e0 >> 1) & 1u, g0 >> 4);
+        a[3] = value(q1 >> 8, (e1 >> 1) & 1u, g1 >> 4);
+        mma_k32<false>(c, a, b);
+      } else {
+        // part s: half s % 2 of slice s / 2. A value less 32 (six bits) is taken as q << 2 with the top bit flipped: four times it, as
+        // a signed byte
+        const int n = s >> 3, q = (s >> 1) & 3, e = s & 1;
+        if ((s & 7) == 0) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {   // slice 4 n + q: nibble q / 2 of ql's half q % 2, bits 2 q of qh
-        const int s = 4 * n + q;
-        auto word = [&](int row, int e) {
-          const uint32_t lo = q < 2 ? l[row][q & 1][e] << 2 : l[row][q & 1][e] >> 2;
-          const uint32_t hi = q == 3 ? h[row][e] : h[row][e] << (6 - 2 * q);
+          for (int i = 0; i < 2; ++i) {
+            h6[0][i] = lds32h(b0 + 128 + 32 * n + 16 * i + 4 * t);
+            h6[1][i] = lds32h(b1 + 128 + 32 * n + 16 * i + 4 * t);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              l6[0][r][i] = lds32h(b0 + 64 * n + 32 * r + 16 * i + 4 * t);
+              l6[1][r][i] = lds32h(b1 + 64 * n + 32 * r + 16 * i + 4 * t);
+            }
+          }
+        }
+        auto word = [&](int row) {     // nibble q / 2 of ql's half q % 2, bits 2 q of qh
+          const uint32_t lo = q < 2 ? l6[row][q & 1][e] << 2 : l6[row][q & 1][e] >> 2;
+          const uint32_t hi = q == 3 ? h6[row][e] : h6[row][e] << (6 - 2 * q);
           return (lo & 0x3C3C3C3Cu) | ((hi & 0xC0C0C0C0u) ^ 0x80808080u);
         };
-        const uint2 b = act_q(x, s);
-        int ca[4], cb[4];
-        mma_k16(ca, word(0, 0), word(1, 0), b.x);
-        mma_k16(cb, word(0, 1), word(1, 1), b.y);
-        const uint32_t s0 = lds16(b0 + 192 + 2 * s), s1 = lds16(b1 + 192 + 2 * s);
-        const int u0 = (int)(int8_t)s0, v0 = (int)(int8_t)(s0 >> 8), u1 = (int)(int8_t)s1, v1 = (int)(int8_t)(s1 >> 8);
-        const float2 d = act_d(x, s);
-        part[0] = fmaf((float)(ca[0] * u0 + cb[0] * v0), d.x, part[0]);
-        part[1] = fmaf((float)(ca[1] * u0 + cb[1] * v0), d.y, part[1]);
-        part[2] = fmaf((float)(ca[2] * u1 + cb[2] * v1), d.x, part[2]);
-        part[3] = fmaf((float)(ca[3] * u1 + cb[3] * v1), d.y, part[3]);
+        mma_k16(c, word(0), word(1), b.x);
       }
     }
-    acc[0] = fmaf(d0, part[0], acc[0]);
-    acc[1] = fmaf(d0, part[1], acc[1]);
-    acc[2] = fmaf(d1, part[2], acc[2]);
-    acc[3] = fmaf(d1, part[3], acc[3]);
+    const float2 d = x.scales(f);
+    const float a00 = row_scale(0, f, 0), a10 = row_scale(1, f, 0), a01 = TT == 1 ? row_scale(0, f, 1) : a00, a11 = TT == 1 ? row_scale(1, f, 1) : a10;
+    acc[0] = fmaf(fmaf(__int_as_float(c[0]), a00, -MAGIC_F * a00), d.x, acc[0]);
+    acc[1] = fmaf(fmaf(__int_as_float(c[1]), a01, -MAGIC_F * a01), d.y, acc[1]);
+    acc[2] = fmaf(fmaf(__int_as_float(c[2]), a10, -MAGIC_F * a10), d.x, acc[2]);
+    acc[3] = fmaf(fmaf(__int_as_float(c[3]), a11, -MAGIC_F * a11), d.y, acc[3]);
+    if constexpr (KIND == Q4K && TT <= 2) {
+      const float n0 = -h2f(h0.x >> 16), n1 = -h2f(h1.x >> 16);
+      const float2 xs = x.quant_sums(f);
+      auto low = [&](int row, int p) {
+        return (row ? n1 : n0) * (byte_on_2_23(mn[row], TT == 1 ? p >= 4 : f, TT == 1 ? p & 3 : p) - 8388608.0f);
+      };
+      const float m00 = low(0, part0), m10 = low(1, part0), m01 = TT == 1 ? low(0, part1) : m00, m11 = TT == 1 ? low(1, part1) : m10;
+      acc[0] = fmaf(m00, xs.x, acc[0]);
+      acc[1] = fmaf(m01, xs.y, acc[1]);
+      acc[2] = fmaf(m10, xs.x, acc[2]);
+      acc[3] = fmaf(m11, xs.y, acc[3]);
+    }
+  }
+  if constexpr (KIND == Q4K && TT >= 4) {
+    // rows g, g + 8 by slices t, t + 4; the sums' columns are the tokens (of 4 tokens, lanes t < 2 have them)
+    auto low = [&](uint32_t w) { return __float_as_uint(__uint_as_float(prmt(w, 0x4B000000u, 0x7440u | t)) - 8388608.0f); };
+    const uint32_t m0 = low(mn[0][0]), m1 = low(mn[1][0]), m2 = low(mn[0][1]), m3 = low(mn[1][1]);
+    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int p = 2; p >= 0; --p) mma_tf32(c, m0, m1, m2, m3, x.minima(p));
+    const float n0 = -h2f(h0.x >> 16), n1 = -h2f(h1.x >> 16);
+    if (TT == 8 || t < 2) {
+      acc[0] = fmaf(n0, c[0], acc[0]);
+      acc[1] = fmaf(n0, c[1], acc[1]);
+      acc[2] = fmaf(n1, c[2], acc[2]);
+      acc[3] = fmaf(n1, c[3], acc[3]);
+    }
+  }
+}
+
+// A lane's sums over the parts that stood side by side: afterwards rows g, g + 8 by tokens 2 t, 2 t + 1.
+template <int TT>
+__device__ __forceinline__ void fold(float (&acc)[4]) {
+  if constexpr (TT == 1) {
+    acc[0] += acc[1];
+    acc[2] += acc[3];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (TT == 1 && (i & 1)) continue;
+    if constexpr (TT <= 2) acc[i] += __shfl_xor_sync(0xFFFFFFFFu, acc[i], 1);
+    if constexpr (TT <= 4) acc[i] += __shfl_xor_sync(0xFFFFFFFFu, acc[i], 2);
   }
 }
 
@@ -253,13 +354,13 @@ __device__ __forceinline__ void load_act(const MoeArgs& a, int pair, int piece, 
 }
 
 // 8 values of column `col` into the staged activations. Whole warps call it: four lanes share a slice of 32 values.
-template <int KIND>
-__device__ __forceinline__ void stage_piece(const float (&v)[8], int piece, int col, uint8_t* q_s, float* d_s, float* min_s) {
+template <int KIND, int CAP>
+__device__ __forceinline__ void stage_piece(const float (&v)[8], int piece, int col, int nsb, uint8_t* q_s, float* d_s, float* min_s) {
   int q[8];
   const float d = moe_quant8(v, q);
   const int s = piece >> 2, p = piece & 3;
   const uint32_t w0 = moe_pack4(q[0], q[1], q[2], q[3]), w1 = moe_pack4(q[4], q[5], q[6], q[7]);
-  uint8_t* to = q_s + 256 * s + 32 * col;
+  uint8_t* to = q_s + (s * CAP + col) * 32;
   if constexpr (KIND == Q6K) {           // lane t's words t and 4 + t side by side
     *reinterpret_cast<uint32_t*>(to + 16 * (p & 1) + 4 * (p >> 1)) = w0;
     *reinterpret_cast<uint32_t*>(to + 16 * (p & 1) + 8 + 4 * (p >> 1)) = w1;
@@ -277,208 +378,210 @@ __device__ __forceinline__ void stage_piece(const float (&v)[8], int piece, int 
     if (p == 0) {                        // d * sum in three parts of at most 11 bits
       const float xs = d * (float)sum, hi = __uint_as_float(__float_as_uint(xs) & 0xFFFFE000u), r = xs - hi;
       const float mid = __uint_as_float(__float_as_uint(r) & 0xFFFFE000u);
-      float* m = min_s + 192 * (s >> 3) + ((s & 3) * 8 + col) * 2 + ((s >> 2) & 1);
+      min_s[s * CAP + col] = xs;
+      float* m = min_s + nsb * 8 * CAP + (s >> 3) * (CAP * 24) + (col * 4 + (s & 3)) * 2 + ((s >> 2) & 1);
       m[0] = hi;
-      m[64] = mid;
-      m[128] = r - mid;
+      m[CAP * 8] = mid;
+      m[CAP * 16] = r - mid;
     }
   }
-  if (p == 0) d_s[8 * s + col] = d;
+  if (p == 0) d_s[s * CAP + col] = d;
 }
 
-// A block's work on one group: tiles [ta, tb), each by `ks` warps along K (k_of: this warp's superblocks).
-struct Segment {
-  int ta, tb, log_ks;
+// A batch: units (group, tile) [u0, u1) of the block's list; first of its groups in the window, and how many.
+struct Batch {
+  int u0, u1, g0, n;
+};
+// The block's range of units, and the window of groups that it is at.
+struct Window {
+  int4 group[WINDOW];        // expert, first place in the list, pairs, first column of the batch's activations
+  Batch batch[WINDOW];
+  int first, batches, end;   // number of the window's first group; one past its last unit
 };
 
-struct Work {
-  int u0, u1, tiles, nsb;      // the block's units; tiles of an expert, superblocks of a row
-  __device__ __forceinline__ int first_group() const { return u0 / tiles; }
-  __device__ __forceinline__ int last_group() const { return (u1 - 1) / tiles; }
-  __device__ __forceinline__ Segment segment(int group) const {
-    Segment s;
-    s.ta = max(u0 - group * tiles, 0);
-    s.tb = min(u1 - group * tiles, tiles);
-    // warps to a tile: rounds over the tiles times superblocks of a warp, and one for the sum where warps share a tile
-    const int n = s.tb - s.ta;
-    int best = 1 << 30;
-    s.log_ks = 0;
-#pragma unroll
-    for (int l = 0; l < 5; ++l) {
-      const int cost = ((n + (WARPS >> l) - 1) / (WARPS >> l)) * (((nsb + (1 << l) - 1) >> l) + (l > 0));
-      if (cost < best) {
-        best = cost;
-        s.log_ks = l;
-      }
-    }
-    return s;
-  }
-};
+// Superblocks s0 .. s1 of a batch are warp `warp`'s.
+__device__ __forceinline__ int chunk_begin(const Batch& b, int nsb, int warp) { return (int)((int64_t)(b.u1 - b.u0) * nsb * warp / WARPS); }
 
-// Where a warp's stream of weights stands: superblocks sb .. of a tile of a group.
-struct Stream {
-  int group, expert, tile, sb, k0, k1, step, tb;
+// A warp's way through the superblocks of its chunks, batch after batch of a window.
+struct Place {
+  int batch, s, s1;          // superblock of the batch, end of the chunk
+  int group, tile, sb;       // group of the window, tile of the group, superblock of the tile
   bool live;
-  __device__ __forceinline__ void enter(const Work& w, const int4* groups, int warp) {   // the first superblocks of `group` or of one behind it
-    for (; group <= w.last_group(); ++group) {
-      const Segment s = w.segment(group);
-      const int kp = warp & ((1 << s.log_ks) - 1);
-      tile = s.ta + (warp >> s.log_ks);
-      k0 = (kp * w.nsb) >> s.log_ks;
-      k1 = ((kp + 1) * w.nsb) >> s.log_ks;
-      step = WARPS >> s.log_ks;
-      tb = s.tb;
-      sb = k0;
-      if (tile < tb && k0 < k1) {
+  __device__ __forceinline__ void enter(const Window& w, int tiles, int nsb, int warp) {   // `batch`, or the next one with work for this warp
+    for (live = false; !live && batch < w.batches; batch += !live) {
+      const Batch b = w.batch[batch];
+      s = chunk_begin(b, nsb, warp);
+      s1 = chunk_begin(b, nsb, warp + 1);
+      if (s < s1) {
         live = true;
-        expert = groups[group].x;
-        return;
+        const int u = s / nsb, at = b.u0 + u;
+        sb = s - u * nsb;
+        group = at / tiles - w.first;
+        tile = at - (group + w.first) * tiles;
       }
     }
-    live = false;
   }
-  __device__ __forceinline__ void next(const Work& w, const int4* groups, int warp, int sbs) {
-    sb += sbs;
-    if (sb < k1) return;
-    sb = k0;
-    tile += step;
-    if (tile < tb) return;
-    ++group;
-    enter(w, groups, warp);
+  // the superblock behind; true where it is another tile's (or there is none left)
+  __device__ __forceinline__ bool next(const Window& w, int tiles, int nsb, int warp) {
+    ++s;
+    ++sb;
+    if (s == s1) {
+      ++batch;
+      enter(w, tiles, nsb, warp);
+      return true;
+    }
+    if (sb < nsb) return false;
+    sb = 0;
+    if (++tile == tiles) {
+      tile = 0;
+      ++group;
+    }
+    return true;
   }
 };
 
-// DOWN: rows of w2 on the activated products, else gate and up rows of w13 on X. `sbs`: superblocks of a stage; `stages`: of a warp's ring.
-template <int KIND, bool DOWN>
-__global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a, int sbs, int stages) {
+// DOWN: rows of w2 on the activated products, else gate and up rows of w13 on X. STAGES: of a warp's ring; CAP: columns of activations.
+template <int KIND, bool DOWN, int STAGES, int CAP>
+__global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int pair_s[8];
+  __shared__ Window win;
+  __shared__ int pair_s[CAP];
+  constexpr int PITCH = pitch(KIND), STAGE = 16 * PITCH, BS = bs(KIND);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int k = DOWN ? a.inter : a.hidden, rows = DOWN ? a.hidden : 2 * a.inter;
+  const int k = DOWN ? a.inter : a.hidden, rows = DOWN ? a.hidden : 2 * a.inter, tiles = rows >> 4, nsb = k >> 8;
   const int64_t rb = DOWN ? a.rb2 : a.rb13;
   const uint8_t* const weights = DOWN ? a.w2 : a.w13;
-  const int row_pitch = sbs == 2 ? pitch(KIND, 2) : pitch(KIND, 1), stage_bytes = 16 * row_pitch;
 
   uint8_t* sp = smem;
   uint8_t* q_s = sp;
-  sp += (size_t)k * 8;
+  sp += (size_t)k * CAP;
   float* d_s = reinterpret_cast<float*>(sp);
-  sp += (size_t)k / 32 * 32;
+  sp += (size_t)k / 32 * CAP * 4;
   float* min_s = reinterpret_cast<float*>(sp);
-  if (KIND == Q4K) sp += (size_t)k / 256 * 768;
+  if (KIND == Q4K) sp += (size_t)k / 256 * CAP * 128;
   uint32_t* grid_s = reinterpret_cast<uint32_t*>(sp);
   if (KIND == IQ3S) sp += 512 * 4 * GRID_COPIES;
-  float4* join_s = reinterpret_cast<float4*>(sp);    // [2][warps][lanes]
+  float4* part_s = reinterpret_cast<float4*>(sp);    // [warps][2][lanes]: sums of a tile that begins before the chunk, that ends behind it
   sp += 2 * WARPS * 512;
-  uint8_t* ring = sp + (size_t)warp * stages * stage_bytes;
-  const uint32_t ring_at = smem_addr(ring), bars = smem_addr(sp + (size_t)WARPS * stages * stage_bytes) + 8 * stages * warp;
-
-  if (lane == 0) {
-    for (int s = 0; s < stages; ++s) bar_init(bars + 8 * s);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  const uint8_t* ring = sp + (size_t)warp * STAGES * STAGE;
+  // a stage's pieces: piece lane + 32 i of 16 rows of PIECES each. Their rows' offsets from row 0 and where they go do not change.
+  constexpr int PIECES = (BS + (KIND == Q4K ? 0 : KIND == IQ4XS ? 8 : 14) + 15) / 16, COPIES = (16 * PIECES + 31) / 32;
+  uint32_t from_row[COPIES], piece_at[COPIES];      // (offset of the piece's row from the tile's first; 16 * piece | slot offset << 8)
+#pragma unroll
+  for (int i = 0; i < COPIES; ++i) {
+    const int c = min(lane + 32 * i, 16 * PIECES - 1), r = c / PIECES, p = c - r * PIECES;
+    from_row[i] = (uint32_t)((DOWN ? r : (r & 7) + (r & 8 ? a.inter : 0)) * rb);
+    piece_at[i] = 16 * p | (r * PITCH + 16 * p) << 8;
   }
-  __syncwarp();
+  const uint32_t copy_to = smem_addr(ring);
 
-  const int groups = *a.groups;
-  Work w;
-  w.tiles = rows >> 4;
-  w.nsb = k >> 8;
-  const int64_t units = (int64_t)groups * w.tiles;
-  w.u0 = (int)(units * blockIdx.x / gridDim.x);
-  w.u1 = (int)(units * (blockIdx.x + 1) / gridDim.x);
-  if (w.u0 == w.u1) return;
-
-  // lane r < 16 copies row r of a stage
-  Stream in{w.first_group(), 0, 0, 0, 0, 0, 0, 0, false};
-  in.enter(w, a.group, warp);
-  auto issue = [&](int slot) {
-    const int n = min(sbs, in.k1 - in.sb);
-    const int r = DOWN ? 16 * in.tile + (lane & 15) : 8 * in.tile + (lane & 7) + (lane & 8 ? a.inter : 0);
-    const int64_t off = ((int64_t)in.expert * rows + r) * rb + in.sb * bs(KIND);
-    const uint32_t bytes = ((uint32_t)(off & 15) + n * bs(KIND) + 15) & ~15u;
-    uint32_t total = lane < 16 ? bytes : 0;
-    total = __reduce_add_sync(0xFFFFFFFFu, total);
-    if (lane == 0) bar_expect(bars + 8 * slot, total);
-    __syncwarp();
-    if (lane < 16) copy_row(ring_at + slot * stage_bytes + lane * row_pitch, weights + (off & ~(int64_t)15), bytes, bars + 8 * slot);
-  };
-  int issued = 0, used = 0;
-  for (; issued < stages && in.live; ++issued) {
-    issue(issued);
-    in.next(w, a.group, warp, sbs);
-  }
+  const int64_t units = (int64_t)*a.groups * tiles;
+  const int block_u1 = (int)(units * (blockIdx.x + 1) / gridDim.x);
+  int u0 = (int)(units * blockIdx.x / gridDim.x);
   if (KIND == IQ3S)
     for (int i = tid; i < 512 * GRID_COPIES; i += THREADS) grid_s[i] = g_iq3s[i / GRID_COPIES];
 
-  for (int group = w.first_group(); group <= w.last_group(); ++group) {
-    const int4 gr = a.group[group];     // expert, first place in the list, pairs
-    const Segment seg = w.segment(group);
-    __syncthreads();                    // the group before is done with the activations
-    if (tid < gr.z) pair_s[tid] = a.list[gr.y + tid];
+  for (; u0 < block_u1; u0 = win.end) {
+    // the window's groups, their columns and batches: a group's first column is even (its scales are read in pairs), and 8 columns from
+    // there on exist
     __syncthreads();
-    {
-      const int per = k >> 3, total = gr.z * per;   // (whole warps: per is a multiple of 32)
-      constexpr int U = 2;
-      for (int i0 = tid; i0 < total; i0 += U * THREADS) {
-        float v[U][8];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int i = i0 + u * THREADS;
-          if (i < total) load_act<DOWN>(a, pair_s[i / per], i % per, v[u]);
+    if (warp == 0) {
+      const int first = u0 / tiles, n = min((block_u1 - 1) / tiles - first + 1, WINDOW);
+      for (int i = lane; i < n; i += 32) win.group[i] = a.group[first + i];
+      __syncwarp();
+      if (lane == 0) {
+        const int end = min(block_u1, (first + n) * tiles);
+        int col = 0, b = 0;
+        win.batch[0] = Batch{u0, end, 0, 0};
+        for (int i = 0; i < n; ++i) {
+          if (col + 8 > CAP) {
+            win.batch[b].u1 = (first + i) * tiles;
+            win.batch[++b] = Batch{(first + i) * tiles, end, i, 0};
+            col = 0;
+          }
+          win.group[i].w = col;
+          ++win.batch[b].n;
+          col += (win.group[i].z + 1) & ~1;
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int i = i0 + u * THREADS;
-          if (i < total) stage_piece<KIND>(v[u], i % per, i / per, q_s, d_s, min_s);
-        }
+        win.first = first;
+        win.batches = b + 1;
+        win.end = end;
       }
     }
     __syncthreads();
-    const int ks = 1 << seg.log_ks, kp = warp & (ks - 1), slot0 = warp >> seg.log_ks;
-    const int k0 = (kp * w.nsb) >> seg.log_ks, k1 = ((kp + 1) * w.nsb) >> seg.log_ks;
-    int turn = 0;
-    for (int tile = seg.ta + slot0; tile < seg.tb; tile += WARPS >> seg.log_ks) {
-      float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (int sb = k0; sb < k1; sb += sbs) {
-        const int slot = used % stages;
-        bar_wait(bars + 8 * slot, (used / stages) & 1);
-        // this lane's rows in the stage, at the offset their copies began before them
-        const int r0 = DOWN ? 16 * tile + g : 8 * tile + g, r1 = DOWN ? r0 + 8 : r0 + a.inter;
-        const int64_t o0 = ((int64_t)gr.x * rows + r0) * rb + sb * bs(KIND), o1 = ((int64_t)gr.x * rows + r1) * rb + sb * bs(KIND);
-        const uint8_t* b0 = ring + slot * stage_bytes + g * row_pitch + (KIND == Q4K ? 0 : (int)(o0 & 15));
-        const uint8_t* b1 = ring + slot * stage_bytes + (g + 8) * row_pitch + (KIND == Q4K ? 0 : (int)(o1 & 15));
-        const int n = min(sbs, k1 - sb);
-        for (int i = 0; i < n; ++i) {
-          const Act x{q_s + (sb + i) * 2048 + 32 * g + 8 * t, d_s + (sb + i) * 64 + 2 * t, min_s + (sb + i) * 192 + (t * 8 + g) * 2};
-          superblock<KIND>(b0 + i * bs(KIND), b1 + i * bs(KIND), x, t, grid_s + (lane & (GRID_COPIES - 1)), acc);
+
+    // the weights' stream
+    Place in;
+    in.batch = 0;
+    in.enter(win, tiles, nsb, warp);
+    int64_t in_off = 0;                // of the tile's first row, at the next superblock
+    auto row_offset = [&](const Place& p, int r) {
+      const int row = DOWN ? 16 * p.tile + r : 8 * p.tile + (r & 7) + (r & 8 ? a.inter : 0);
+      return ((int64_t)win.group[p.group].x * rows + row) * rb + p.sb * BS;
+    };
+    if (in.live) in_off = row_offset(in, 0);
+    auto issue = [&](int slot) {       // one stage's copies; an empty group of copies where there is nothing left
+      if (in.live) {
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i) {
+          if (32 * i + 31 >= 16 * PIECES && lane + 32 * i >= 16 * PIECES) continue;
+          const uint32_t p = piece_at[i] & 255u;
+          const uint32_t to = copy_to + slot * STAGE + (piece_at[i] >> 8);
+          const int64_t off = in_off + from_row[i];
+          if (KIND == Q4K) copy16(to, weights + off + p);
+          else if (p < (uint32_t)(off & 15) + BS) copy16(to, weights + (off & ~(int64_t)15) + p);
         }
-        ++used;
-        __syncwarp();                   // all lanes have read the stage
-        if (in.live) {
-          issue(slot);
-          ++issued;
-          in.next(w, a.group, warp, sbs);
-        }
+        in_off += BS;
+        if (in.next(win, tiles, nsb, warp) && in.live) in_off = row_offset(in, 0);
       }
-      if (ks > 1) {
-        float4* buf = join_s + turn * WARPS * 32;
-        turn ^= 1;                      // (the other buffer's readers have passed this tile's barrier by the next but one)
-        buf[warp * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-        warps_sync(1 + slot0, 32 * ks);
-        if (kp == 0) {
-          for (int i = 1; i < ks; ++i) {
-            const float4 o = buf[(warp + i) * 32 + lane];
-            acc[0] += o.x; acc[1] += o.y; acc[2] += o.z; acc[3] += o.w;
+      commit();
+    };
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) issue(s);
+
+    Place at;
+    at.batch = 0;
+    at.enter(win, tiles, nsb, warp);
+    int slot = 0;
+    for (int batch = 0; batch < win.batches; ++batch) {
+      const Batch bt = win.batch[batch];
+      {
+        // columns of the batch: pairs, then their rows' values (unused columns in between hold what was there)
+        __syncthreads();                // the batch before is done with them
+        if (tid < CAP) pair_s[tid] = -1;
+        __syncthreads();
+        if (tid < bt.n * 8) {
+          const int4 gr = win.group[bt.g0 + (tid >> 3)];
+          if ((tid & 7) < gr.z) pair_s[gr.w + (tid & 7)] = a.list[gr.y + (tid & 7)];
+        }
+        __syncthreads();
+        const int per = k >> 3, last = win.group[bt.g0 + bt.n - 1].w + win.group[bt.g0 + bt.n - 1].z, total = last * per;   // (whole warps: per % 32 == 0)
+        constexpr int U = 2;
+        for (int i0 = tid; i0 < total; i0 += U * THREADS) {
+          float v[U][8];
+          int pair[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * THREADS;
+            pair[u] = i < total ? pair_s[i / per] : -1;
+            if (pair[u] >= 0) load_act<DOWN>(a, pair[u], i % per, v[u]);
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * THREADS;
+            if (pair[u] >= 0) stage_piece<KIND, CAP>(v[u], i % per, i / per, nsb, q_s, d_s, min_s);
           }
         }
+        __syncthreads();
       }
-      if (kp == 0) {
+      // stores a tile's sums: rows g, g + 8 by columns 2 t, 2 t + 1 of the group
+      auto finish = [&](const float (&acc)[4], int group, int tile) {
+        const int4 gr = win.group[group];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const int col = 2 * t + c;
           if (col < gr.z) {
-            const int pair = pair_s[col];
+            const int pair = pair_s[gr.w + col];
             if constexpr (DOWN) {
               float* to = a.part + (int64_t)pair * a.hidden + 16 * tile + g;
               const float wt = a.weights[pair];
@@ -489,6 +592,69 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a, in
             }
           }
         }
+      };
+      int open_unit = -1, open_group = 0, open_tile = 0;   // the tile that this warp has the beginning of, but not the end
+      while (at.live && at.batch == batch) {
+        // a tile, or this warp's part of one
+        const int group = at.group, tile = at.tile, unit = bt.u0 + at.s / nsb;
+        const bool begins = at.sb == 0;
+        const int4 gr = win.group[group];
+        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        uint32_t p0 = 0, p1 = 0;        // a row begins in its stage at what its offset is past a 16-byte boundary
+        if (KIND != Q4K) {
+          p0 = (uint32_t)row_offset(at, g);
+          p1 = (uint32_t)row_offset(at, g + 8);
+        }
+        bool ends = false;
+        auto run = [&](auto tokens) {
+          constexpr int TT = decltype(tokens)::value;
+          Act<KIND, CAP, TT> x(q_s, d_s, min_s, nsb, at.sb, gr.w, g, t);
+          bool more = true;
+          do {
+            wait_all_but<STAGES - 2>();
+            __syncwarp();               // every lane's pieces are there, and every lane is done with the stage before
+            issue(slot == 0 ? STAGES - 1 : slot - 1);
+            const uint8_t* b0 = ring + slot * STAGE + g * PITCH + (KIND == Q4K ? 0 : p0 & 15);
+            const uint8_t* b1 = ring + slot * STAGE + (g + 8) * PITCH + (KIND == Q4K ? 0 : p1 & 15);
+            superblock<KIND, CAP, TT>(b0, b1, x, g, t, grid_s + (lane & (GRID_COPIES - 1)), acc);
+            x.next();
+            p0 += BS;
+            p1 += BS;
+            if (++slot == STAGES) slot = 0;
+            ends = at.sb == nsb - 1;
+            more = !at.next(win, tiles, nsb, warp);
+          } while (more);
+          fold<TT>(acc);
+        };
+        if (gr.z == 1) run(std::integral_constant<int, 1>());
+        else if (gr.z == 2) run(std::integral_constant<int, 2>());
+        else if (gr.z <= 4) run(std::integral_constant<int, 4>());
+        else run(std::integral_constant<int, 8>());
+        if (begins && ends) {
+          finish(acc, group, tile);
+        } else {
+          part_s[(2 * warp + begins) * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+          if (begins) {
+            open_unit = unit;
+            open_group = group;
+            open_tile = tile;
+          }
+        }
+      }
+      __syncthreads();                  // all parts are there, and nobody reads the activations any more
+      if (open_unit >= 0) {
+        const int tile_end = (open_unit - bt.u0 + 1) * nsb;
+        float4 v = part_s[(2 * warp + 1) * 32 + lane];
+        for (int o = warp + 1, from = chunk_begin(bt, nsb, o); from < tile_end; ++o) {
+          const int to = chunk_begin(bt, nsb, o + 1);
+          if (to > from) {
+            const float4 q = part_s[2 * o * 32 + lane];
+            v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+          }
+          from = to;
+        }
+        const float acc[4] = {v.x, v.y, v.z, v.w};
+        finish(acc, open_group, open_tile);
       }
     }
   }
@@ -498,31 +664,35 @@ static int kind_of(int type) {
   return type == GSQ_TYPE_Q4_K ? Q4K : type == GSQ_TYPE_Q6_K ? Q6K : type == GSQ_TYPE_IQ3_S ? IQ3S : type == GSQ_TYPE_IQ4_XS ? IQ4XS : -1;
 }
 
-// Superblocks of a stage and stages of a warp's ring that fit beside a row length of k: two superblocks a copy where that leaves two
-// stages or more, at most four stages. False: too long a row.
-static bool ring_of(int kind, int k, int max_smem, int* sbs, int* stages, size_t* smem) {
-  const size_t fixed = fixed_smem(kind, k);
-  for (int s = kind == Q6K ? 1 : 2; s >= 1; --s) {
-    const size_t stage = (size_t)WARPS * (16 * pitch(kind, s) + 8);
-    if (fixed + 2 * stage > (size_t)max_smem - 1024) continue;
-    const size_t n = ((size_t)max_smem - 1024 - fixed) / stage;
-    *sbs = s;
-    *stages = (int)(n < 4 ? n : 4);
-    *smem = fixed + *stages * stage;
-    return true;
+// Columns of activations and stages of a warp's ring beside rows of k values. False: too long a row.
+static bool plan_of(int kind, int k, int max_smem, int* cap, int* stages, size_t* smem) {
+  const size_t room = (size_t)max_smem - 4096, stage = (size_t)WARPS * 16 * pitch(kind);   // (4096: the window and the driver's own)
+  const int plans[4][2] = {{16, 4}, {16, 3}, {8, 4}, {8, 2}};
+  for (const auto& p : plans) {
+    *cap = p[0];
+    *stages = p[1];
+    *smem = fixed_smem(kind, k, p[0]) + p[1] * stage;
+    if (*smem <= room) return true;
   }
   return false;
 }
 
-template <int KIND, bool DOWN>
-static int launch(const MoeArgs& a, const DeviceInfo& di, cudaStream_t st) {
-  int sbs, stages;
-  size_t smem;
-  if (!ring_of(KIND, DOWN ? a.inter : a.hidden, di.max_smem_optin, &sbs, &stages, &smem)) return GSQ_ERR_UNSUPPORTED;
-  GSQ_CUDA_TRY(cudaFuncSetAttribute(moe_mma_kernel<KIND, DOWN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  moe_mma_kernel<KIND, DOWN><<<di.sm_count, THREADS, smem, st>>>(a, sbs, stages);
+template <int KIND, bool DOWN, int STAGES, int CAP>
+static int launch_kernel(const MoeArgs& a, size_t smem, int blocks, cudaStream_t st) {
+  GSQ_CUDA_TRY(cudaFuncSetAttribute(moe_mma_kernel<KIND, DOWN, STAGES, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  moe_mma_kernel<KIND, DOWN, STAGES, CAP><<<blocks, THREADS, smem, st>>>(a);
   GSQ_CUDA_TRY(cudaGetLastError());
   return GSQ_OK;
+}
+
+template <int KIND, bool DOWN>
+static int launch(const MoeArgs& a, const DeviceInfo& di, cudaStream_t st) {
+  int cap, stages;
+  size_t smem;
+  if (!plan_of(KIND, DOWN ? a.inter : a.hidden, di.max_smem_optin, &cap, &stages, &smem)) return GSQ_ERR_UNSUPPORTED;
+  return cap == 16     ? (stages == 4 ? launch_kernel<KIND, DOWN, 4, 16>(a, smem, di.sm_count, st) : launch_kernel<KIND, DOWN, 3, 16>(a, smem, di.sm_count, st))
+         : stages == 4 ? launch_kernel<KIND, DOWN, 4, 8>(a, smem, di.sm_count, st)
+                       : launch_kernel<KIND, DOWN, 2, 8>(a, smem, di.sm_count, st);
 }
 
 }  // namespace moe
@@ -531,9 +701,9 @@ static int launch(const MoeArgs& a, const DeviceInfo& di, cudaStream_t st) {
 bool moe_mma_serves(int type, int k) {
   const int kind = moe::kind_of(type);
   DeviceInfo di;
-  int sbs, stages;
+  int cap, stages;
   size_t smem;
-  return kind >= 0 && device_info(&di) == GSQ_OK && moe::ring_of(kind, k, di.max_smem_optin, &sbs, &stages, &smem);
+  return kind >= 0 && device_info(&di) == GSQ_OK && moe::plan_of(kind, k, di.max_smem_optin, &cap, &stages, &smem);
 }
 
 int moe_mma_product(const MoeArgs& a, int type, bool down, cudaStream_t st) {
@@ -550,11 +720,6 @@ int moe_mma_product(const MoeArgs& a, int type, bool down, cudaStream_t st) {
     default: return GSQ_ERR_UNSUPPORTED;
   }
 #undef GSQ_MOE_KIND
-}
-
-int moe_error_flag(int* flag) {
-  GSQ_CUDA_TRY(cudaMemcpyFromSymbol(flag, moe::g_error, sizeof(int)));
-  return GSQ_OK;
 }
 
 }  // namespace gsq
