@@ -20,12 +20,6 @@ __device__ __forceinline__ uint32_t score_key(float v) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-__device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
-  return dtype == GSQ_F32 ? reinterpret_cast<const float*>(p)[i]
-         : dtype == GSQ_F16 ? __half2float(reinterpret_cast<const __half*>(p)[i])
-                            : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
-}
-
 constexpr int ROUTE_PER_LANE = GSQ_MOE_MAX_EXPERTS / 32;
 
 struct RouteArgs {
@@ -45,10 +39,24 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int token, int l
   float s[PER_LANE];
   uint32_t key[PER_LANE];
   float top = -INFINITY;
+  // (one branch on the type around all loads: they are under way together)
+  const int64_t row = token * a.stride;
+  if (a.dtype == GSQ_F32) {
+#pragma unroll
+    for (int i = 0; i < PER_LANE; ++i) s[i] = lane + 32 * i < a.experts ? reinterpret_cast<const float*>(a.logits)[row + lane + 32 * i] : -INFINITY;
+  } else {
+    uint16_t raw[PER_LANE];
+#pragma unroll
+    for (int i = 0; i < PER_LANE; ++i) raw[i] = lane + 32 * i < a.experts ? reinterpret_cast<const uint16_t*>(a.logits)[row + lane + 32 * i] : 0;
+#pragma unroll
+    for (int i = 0; i < PER_LANE; ++i)
+      s[i] = lane + 32 * i >= a.experts ? -INFINITY
+             : a.dtype == GSQ_F16       ? __half2float(__ushort_as_half(raw[i]))
+                                        : __uint_as_float((uint32_t)raw[i] << 16);
+  }
 #pragma unroll
   for (int i = 0; i < PER_LANE; ++i) {
-    const int e = lane + 32 * i;
-    const float z = e < a.experts ? load_any(a.logits, a.dtype, token * a.stride + e) : -INFINITY;
+    const float z = s[i];
     s[i] = isnan(z) ? -INFINITY : fminf(z, 3.402823466e38f);   // experts at +inf share the weight
     key[i] = score_key(s[i]);
     top = fmaxf(top, s[i]);
@@ -129,11 +137,11 @@ static int launch_route(const RouteArgs& a, cudaStream_t st) {
   return GSQ_OK;
 }
 
-// Rows of k values -> 8-bit form. One thread takes 8 values.
+// Rows of k values -> 8-bit form. One thread takes 8 values; `i`: which.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) moe_quant_kernel(const void* x, int64_t stride, int64_t rows, int k, int8_t* q8, float* d8) {
+__device__ __forceinline__ void quant_piece(const void* x, int64_t stride, int64_t rows, int k, int8_t* q8, float* d8, int64_t i) {
   const int per_row = k >> 3;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / per_row;
+  const int64_t row = i / per_row;
   const int c = (int)(i - row * per_row);
   float v[8] = {};
   if (row < rows) load8<T, VEC>(reinterpret_cast<const T*>(x), row * stride + 8 * c, v);
@@ -143,6 +151,10 @@ __global__ void __launch_bounds__(256) moe_quant_kernel(const void* x, int64_t s
     *reinterpret_cast<uint2*>(q8 + row * k + 8 * c) = make_uint2(moe_pack4(q[0], q[1], q[2], q[3]), moe_pack4(q[4], q[5], q[6], q[7]));
     if ((c & 3) == 0) d8[row * (k >> 5) + (c >> 2)] = d;
   }
+}
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) moe_quant_kernel(const void* x, int64_t stride, int64_t rows, int k, int8_t* q8, float* d8) {
+  quant_piece<T, VEC>(x, stride, rows, k, q8, d8, (int64_t)blockIdx.x * 256 + threadIdx.x);
 }
 
 static int launch_quant(const void* x, int dtype, int vec, int64_t stride, int64_t rows, int k, int8_t* q8, float* d8, cudaStream_t st) {
@@ -163,6 +175,7 @@ static int launch_quant(const void* x, int dtype, int vec, int64_t stride, int64
 
 // y = sum of a token's parts, in the order of its choices.
 __global__ void __launch_bounds__(256) moe_combine_kernel(const MoeArgs a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int per_row = a.hidden >> 2;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, t = i / per_row;
   if (t >= a.m) return;
@@ -181,45 +194,124 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(const MoeArgs a) {
   store_out_dyn(a.y, a.x_dtype, at + 3, s.w);
 }
 
-// Pairs by expert: group, list. One block. An expert's pairs stay in their order, so that the same ones share a group every time (a
-// group's size decides the order of its sums).
-constexpr int PLAN_THREADS = 1024;
-__global__ void __launch_bounds__(PLAN_THREADS) moe_plan_kernel(const MoeArgs a) {
-  __shared__ int count[GSQ_MOE_MAX_EXPERTS], place[GSQ_MOE_MAX_EXPERTS];
-  __shared__ int2 warp_sum[PLAN_THREADS / 32];
-  __shared__ uint8_t of_warp[PLAN_THREADS / 32][GSQ_MOE_MAX_EXPERTS];   // pairs of an expert among a warp's 32
-  const int tid = threadIdx.x, lane = tid & 31, pairs = a.m * a.top_k;
-  count[tid] = 0;
-  __syncthreads();
-  for (int p = tid; p < pairs; p += PLAN_THREADS) {
-    const int e = moe_expert(a, p);
-    if (e >= 0) atomicAdd(&count[e], 1);
+// What a tile of groups of n pairs costs (in 16ths of one of a single token): instructions of the tensor-core kernel.
+__device__ __forceinline__ int moe_cost(int n) {
+  const int r = n & 7;
+  return (n >> 3) * 28 + (r == 0 ? 0 : r == 1 ? 16 : r == 2 ? 17 : r <= 4 ? 21 : 28);
+}
+
+// Pairs by expert: group, list, bounds. Block 0; PER_LANE > 0: it makes the choice first (few tokens). An expert's pairs stay in
+// their order, so that the same ones share a group every time (a group's size decides the order of its sums). Everything behind it
+// waits for it, so it is kept short: per warp of pairs the equal ones are found by matching, and the rest are sums over the
+// warps, the experts, and a search per block of the products.
+constexpr int PLAN_THREADS = 1024, PLAN_WARPS = PLAN_THREADS / 32;
+template <int PER_LANE>
+__global__ void __launch_bounds__(PLAN_THREADS) moe_plan_kernel(const MoeArgs a, const RouteArgs r) {
+  __shared__ uint8_t of_warp[PLAN_WARPS][GSQ_MOE_MAX_EXPERTS];   // an expert's pairs among a warp's 32
+  __shared__ int place[GSQ_MOE_MAX_EXPERTS], cost_upto[GSQ_MOE_MAX_EXPERTS], group_upto[GSQ_MOE_MAX_EXPERTS];
+  __shared__ int3 warp_sum[PLAN_WARPS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, pairs = a.m * a.top_k, experts = a.experts;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (blockIdx.x > 0) {                                          // the other blocks quantise X meanwhile
+
+    const int64_t i = (int64_t)(blockIdx.x - 1) * PLAN_THREADS + tid;
+    if (a.x_dtype == GSQ_F32) {
+      if (a.x_vec) quant_piece<float, true>(a.x, a.x_stride, a.m, a.hidden, a.xq, a.xd, i);
+      else quant_piece<float, false>(a.x, a.x_stride, a.m, a.hidden, a.xq, a.xd, i);
+    } else if (a.x_dtype == GSQ_F16) {
+      if (a.x_vec) quant_piece<__half, true>(a.x, a.x_stride, a.m, a.hidden, a.xq, a.xd, i);
+      else quant_piece<__half, false>(a.x, a.x_stride, a.m, a.hidden, a.xq, a.xd, i);
+    } else {
+      if (a.x_vec) quant_piece<__nv_bfloat16, true>(a.x, a.x_stride, a.m, a.hidden, a.xq, a.xd, i);
+      else quant_piece<__nv_bfloat16, false>(a.x, a.x_stride, a.m, a.hidden, a.xq, a.xd, i);
+    }
+    return;
   }
+  const int warps = min((pairs + 31) >> 5, PLAN_WARPS);           // that have pairs
+  for (int w = 0; w < warps; ++w)
+    if (tid < experts) of_warp[w][tid] = 0;
+  if constexpr (PER_LANE > 0)
+    for (int t = warp; t < a.m; t += PLAN_WARPS) route_token<PER_LANE>(r, t, lane);
   __syncthreads();
-  // places of the experts in the list and of their groups: sums over the experts before
-  const int n = count[tid], g = (n + 7) >> 3;
-  int2 upto = make_int2(n, g);
+
+  const bool once = pairs <= PLAN_THREADS;
+  int expert = -1, rank = 0, n = 0;
+  if (once) {
+    if (warp < warps) {
+      expert = tid < pairs ? moe_expert(a, tid) : -1;
+      const uint32_t same = __match_any_sync(0xFFFFFFFFu, expert);
+      rank = __popc(same & ((1u << lane) - 1));
+      if (expert >= 0 && rank == 0) of_warp[warp][expert] = (uint8_t)__popc(same);
+    }
+    __syncthreads();
+    if (tid < experts)
+      for (int w = 0; w < warps; ++w) n += of_warp[w][tid];
+  } else {
+    place[tid] = 0;
+    __syncthreads();
+    for (int p = tid; p < pairs; p += PLAN_THREADS) {
+      const int e = moe_expert(a, p);
+      if (e >= 0) atomicAdd(&place[e], 1);
+    }
+    __syncthreads();
+    n = place[tid];
+    __syncthreads();
+  }
+  // sums over the experts before: pairs, groups, cost
+  const int g = (n + 7) >> 3, cost = moe_cost(n);
+  int3 upto = make_int3(n, g, cost);
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xFFFFFFFFu, upto.x, o), y = __shfl_up_sync(0xFFFFFFFFu, upto.y, o);
+    const int x = __shfl_up_sync(0xFFFFFFFFu, upto.x, o), y = __shfl_up_sync(0xFFFFFFFFu, upto.y, o), z = __shfl_up_sync(0xFFFFFFFFu, upto.z, o);
     if (lane >= o) {
       upto.x += x;
       upto.y += y;
+      upto.z += z;
     }
   }
-  if (lane == 31) warp_sum[tid >> 5] = upto;
+  if (lane == 31) warp_sum[warp] = upto;
   __syncthreads();
-  for (int w = 0; w < (tid >> 5); ++w) {
-    upto.x += warp_sum[w].x;
-    upto.y += warp_sum[w].y;
-  }
+  const int3 other = warp_sum[lane];
+  const uint32_t mine = 0xFFFFFFFFu;
+  upto.x += __reduce_add_sync(mine, lane < warp ? other.x : 0);
+  upto.y += __reduce_add_sync(mine, lane < warp ? other.y : 0);
+  upto.z += __reduce_add_sync(mine, lane < warp ? other.z : 0);
+  const int groups = __reduce_add_sync(mine, other.y), total = __reduce_add_sync(mine, other.z);
   place[tid] = upto.x - n;
+  cost_upto[tid] = upto.z;
+  group_upto[tid] = upto.y;
   for (int i = 0; i < g; ++i) a.group[upto.y - g + i] = make_int4(tid, upto.x - n + 8 * i, min(8, n - 8 * i), 0);
-  if (tid == PLAN_THREADS - 1) *a.groups = upto.y;
-  const int warp = tid >> 5;
+  __syncthreads();
+
+  // block b of the products begins at cost total * b / blocks: in the first expert whose groups end behind that
+  for (int b = tid; b <= a.blocks; b += PLAN_THREADS) {
+    int2 at = make_int2(groups, 0);
+    if (b < a.blocks && total > 0) {
+      const int target = (int)((uint32_t)total * b / a.blocks);   // (at most 32768 * 28 * 256 / 8)
+      int lo = 0, hi = experts - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (cost_upto[mid] > target) hi = mid;
+        else lo = mid + 1;
+      }
+      // its groups: full ones of moe_cost(8), then the rest
+      const int first = lo ? group_upto[lo - 1] : 0, in = target - (lo ? cost_upto[lo - 1] : 0);
+      const int i = min(in / moe_cost(8), group_upto[lo] - first - 1), rest = in - i * moe_cost(8);
+      const int whole = min(moe_cost(8), cost_upto[lo] - (lo ? cost_upto[lo - 1] : 0) - i * moe_cost(8));
+      at = make_int2(first + i, (rest << 16) / whole);
+    }
+    a.bounds[b] = at;
+  }
+  if (once) {
+    if (expert >= 0) {
+      for (int w = 0; w < warp; ++w) rank += of_warp[w][expert];
+      a.list[place[expert] + rank] = tid;
+    }
+    return;
+  }
   for (int p0 = 0; p0 < pairs; p0 += PLAN_THREADS) {
     const int p = p0 + tid, e = p < pairs ? moe_expert(a, p) : -1;
-    for (int i = lane; i < a.experts; i += 32) of_warp[warp][i] = 0;
+    for (int i = lane; i < experts; i += 32) of_warp[warp][i] = 0;
     __syncwarp();
     const uint32_t same = __match_any_sync(0xFFFFFFFFu, e);
     if (e >= 0 && lane == __ffs(same) - 1) of_warp[warp][e] = (uint8_t)__popc(same);
@@ -230,8 +322,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) moe_plan_kernel(const MoeArgs a)
       a.list[at] = p;
     }
     __syncthreads();
-    if (tid < a.experts)
-      for (int w = 0; w < PLAN_THREADS / 32; ++w) place[tid] += of_warp[w][tid];
+    if (tid < experts)
+      for (int w = 0; w < PLAN_WARPS; ++w) place[tid] += of_warp[w][tid];
     __syncthreads();
   }
 }
@@ -250,14 +342,14 @@ struct Pieces {
   }
 };
 struct MoeLayout {
-  size_t weights, ids, groups, group, list, xq, xd, h, hq, hd, part, total;
+  size_t weights, ids, bounds, group, list, xq, xd, h, hq, hd, part, total;
   MoeLayout(int64_t m, int64_t hidden, int64_t inter, int top_k) {
     Pieces p;
     weights = p.next((size_t)m * top_k * 4);
     ids = p.next((size_t)m * top_k * 4);
     m = m < PASS_TOKENS ? m : PASS_TOKENS;
     const size_t pairs = (size_t)m * top_k;
-    groups = p.next(4);
+    bounds = p.next((MOE_BLOCKS + 1) * 8);
     group = p.next(pairs * 16);
     list = p.next(pairs * 4);
     xq = p.next((size_t)m * hidden);
@@ -298,8 +390,23 @@ static int check_moe(const gsq_moe* w, const void* x, int x_dtype, int64_t m, in
   return GSQ_OK;
 }
 
+// Up to this many tokens and experts the plan's one block makes the choice as well (a warp takes two tokens; more experts than 8 a lane
+// do not fit its registers), which saves a launch.
+constexpr int64_t PLAN_ROUTES = 64, PLAN_EXPERTS = 256;
+
+static int launch_plan(const MoeArgs& a, const RouteArgs* r, cudaStream_t st) {
+  const unsigned grid = 1 + (unsigned)(((int64_t)a.m * (a.hidden >> 3) + PLAN_THREADS - 1) / PLAN_THREADS);
+  if (!r) moe_plan_kernel<0><<<grid, PLAN_THREADS, 0, st>>>(a, RouteArgs{});
+  else if (a.experts <= 64) moe_plan_kernel<2><<<grid, PLAN_THREADS, 0, st>>>(a, *r);
+  else if (a.experts <= 128) moe_plan_kernel<4><<<grid, PLAN_THREADS, 0, st>>>(a, *r);
+  else moe_plan_kernel<8><<<grid, PLAN_THREADS, 0, st>>>(a, *r);
+  GSQ_CUDA_TRY(cudaGetLastError());
+  return GSQ_OK;
+}
+
+// route: the choice to be made here, or NULL where ids and weights are there.
 static int run_experts(const gsq_moe* w, const void* x, int x_dtype, int64_t m, int64_t x_row_stride, const float* weights, const void* ids,
-                       int ids64, int top_k, void* y, int64_t y_row_stride, uint8_t* ws, cudaStream_t st) {
+                       int ids64, int top_k, void* y, int64_t y_row_stride, uint8_t* ws, const RouteArgs* route, cudaStream_t st) {
   const MoeLayout l(m, w->hidden, w->inter, top_k);
   MoeArgs a;
   a.w13 = (const uint8_t*)w->w13;
@@ -317,7 +424,11 @@ static int run_experts(const gsq_moe* w, const void* x, int x_dtype, int64_t m, 
   a.x_vec = (uintptr_t)x % 16 == 0 && (m == 1 || x_row_stride * es % 16 == 0);
   a.ids64 = ids64;
   a.y_stride = y_row_stride;
-  a.groups = (int*)(ws + l.groups);
+  a.bounds = (int2*)(ws + l.bounds);
+  DeviceInfo di;
+  const int rc0 = device_info(&di);
+  if (rc0 != GSQ_OK) return rc0;
+  a.blocks = di.sm_count < MOE_BLOCKS ? di.sm_count : MOE_BLOCKS;
   a.group = (int4*)(ws + l.group);
   a.list = (int*)(ws + l.list);
   a.xq = (int8_t*)(ws + l.xq);
@@ -334,14 +445,15 @@ static int run_experts(const gsq_moe* w, const void* x, int x_dtype, int64_t m, 
     a.weights = weights + t0 * top_k;
     a.ids = (const uint8_t*)ids + t0 * top_k * id_bytes;
     int rc = GSQ_OK;
-    if (up_mma || down_mma) {
-      moe_plan_kernel<<<1, PLAN_THREADS, 0, st>>>(a);
-      GSQ_CUDA_TRY(cudaGetLastError());
-    }
+    const bool plan = up_mma || down_mma;
+    const bool plan_routes = route && plan && m <= PLAN_ROUTES && a.experts <= PLAN_EXPERTS;
+    if (route && t0 == 0 && !plan_routes) rc = launch_route(*route, st);
+    if (rc == GSQ_OK && plan) rc = launch_plan(a, plan_routes ? route : nullptr, st);
+    if (rc != GSQ_OK) return rc;
     if (up_mma) {
       rc = moe_mma_product(a, w->w13_type, false, st);
     } else {
-      rc = launch_quant(a.x, x_dtype, a.x_vec, x_row_stride, a.m, a.hidden, a.xq, a.xd, st);
+      if (!plan) rc = launch_quant(a.x, x_dtype, a.x_vec, x_row_stride, a.m, a.hidden, a.xq, a.xd, st);
       if (rc == GSQ_OK) rc = moe_dot_gate_up(a, w->w13_type, st);
     }
     if (rc != GSQ_OK) return rc;
@@ -352,8 +464,8 @@ static int run_experts(const gsq_moe* w, const void* x, int x_dtype, int64_t m, 
       if (rc == GSQ_OK) rc = moe_dot_down(a, w->w2_type, st);
     }
     if (rc != GSQ_OK) return rc;
-    moe_combine_kernel<<<(unsigned)(((int64_t)a.m * (a.hidden >> 2) + 255) / 256), 256, 0, st>>>(a);
-    GSQ_CUDA_TRY(cudaGetLastError());
+    rc = moe_launch_behind(moe_combine_kernel, (unsigned)(((int64_t)a.m * (a.hidden >> 2) + 255) / 256), 256, 0, st, a);
+    if (rc != GSQ_OK) return rc;
   }
   return GSQ_OK;
 }
@@ -381,7 +493,7 @@ extern "C" int gsq_moe_experts(const gsq_moe* w, const void* x, int x_dtype, int
   if (rc != GSQ_OK || m == 0) return rc;
   if (!topk_weights || !topk_ids) return GSQ_ERR_UNSUPPORTED;
   return gsq::run_experts(w, x, x_dtype, m, x_row_stride, topk_weights, topk_ids, ids_64, top_k, y, y_row_stride, (uint8_t*)workspace,
-                          (cudaStream_t)stream);
+                          nullptr, (cudaStream_t)stream);
 }
 
 extern "C" int gsq_moe_layer(const gsq_moe* w, const void* x, int x_dtype, int64_t m, int64_t x_row_stride, const gsq_moe_router* r, int top_k,
@@ -394,7 +506,6 @@ extern "C" int gsq_moe_layer(const gsq_moe* w, const void* x, int x_dtype, int64
   uint8_t* ws = (uint8_t*)workspace;
   float* weights = (float*)(ws + l.weights);
   int32_t* ids = (int32_t*)(ws + l.ids);
-  rc = gsq::launch_route(gsq::route_args(r, m, w->experts, top_k, weights, ids), (cudaStream_t)stream);
-  if (rc != GSQ_OK) return rc;
-  return gsq::run_experts(w, x, x_dtype, m, x_row_stride, weights, ids, 0, top_k, y, y_row_stride, ws, (cudaStream_t)stream);
+  const gsq::RouteArgs route = gsq::route_args(r, m, w->experts, top_k, weights, ids);
+  return gsq::run_experts(w, x, x_dtype, m, x_row_stride, weights, ids, 0, top_k, y, y_row_stride, ws, &route, (cudaStream_t)stream);
 }

@@ -6,6 +6,8 @@
 
 namespace gsq {
 
+constexpr int MOE_BLOCKS = 256;   // most blocks of a product (one an SM)
+
 struct MoeArgs {
   const uint8_t *w13, *w2;     // [experts][2 inter][row bytes], [experts][hidden][row bytes], GGUF order
   int64_t rb13, rb2;           // bytes of a row
@@ -26,34 +28,42 @@ struct MoeArgs {
   float* h;                    // [pairs][inter]: act(gate) * up
   float* part;                 // [pairs][hidden]: weight times down product
   // pairs by expert, at most 8 to a group
-  int* groups;                 // how many
+  int2* bounds;                // [blocks + 1]: where a block's share of (group, tile) begins: a group, and 65536ths of its tiles
+  int blocks;                  // of the products
   int4* group;                 // expert, first place in the list, pairs
   int* list;                   // pairs
 };
 
 // Expert of a pair, -1 for one that is not here (negative or past the last).
 __device__ __forceinline__ int moe_expert(const MoeArgs& a, int pair) {
-  const int64_t e = a.ids64 ? __ldg(reinterpret_cast<const long long*>(a.ids) + pair) : (int64_t)__ldg(reinterpret_cast<const int*>(a.ids) + pair);
+  // (not the read-only path: the block that plans may have made the choice itself)
+  const int64_t e = a.ids64 ? reinterpret_cast<const long long*>(a.ids)[pair] : (int64_t) reinterpret_cast<const int*>(a.ids)[pair];
   return e >= 0 && e < a.experts ? (int)e : -1;
 }
 
 // q = round(127 x / amax), ties away from zero, of 8 of the 32 values that 4 adjacent lanes share; returns the scale amax / 127.
-// The product 127 x is exact for 16-bit x, so that a quotient that is half an integer is recognised (x / (amax / 127) rounds
-// twice before it rounds to an integer). NaN or an infinity in the block makes the scale NaN or infinite, and so the product NaN.
-// Whole warps call it.
+// The quotient is formed with an approximate reciprocal, and whether it reaches the half-integer that it is next to is decided by
+// the sign of 127 |x| - half * amax in one fused step, which is exact for 16-bit x (127 x is then exact): the result is that of
+// the correctly rounded quotient. (Eight divisions a lane took three times as long: 10 of 16 us of a block's 8 x 5120 activations.)
+// NaN or an infinity in the block makes the scale NaN or infinite, and so the product NaN. Whole warps call it.
 __device__ __forceinline__ float moe_quant8(const float (&v)[8], int (&q)[8]) {
   float amax = 0.0f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) asm("max.NaN.f32 %0, %1, %2;" : "=f"(amax) : "f"(amax), "f"(fabsf(v[e])));
 #pragma unroll
   for (int o = 2; o > 0; o >>= 1) asm("max.NaN.f32 %0, %1, %2;" : "=f"(amax) : "f"(amax), "f"(__shfl_xor_sync(0xFFFFFFFFu, amax, o)));
-  const float s = amax > 1e36f ? 0x1p-10f : 1.0f, den = amax * s;   // 127 x stays finite
+  // 127 x and the reciprocal far from overflow and from 0 (a block of zeros stays zeros: 0 < half * amax)
+  float s = 1.0f;
+  if (!(amax > 1e-30f && amax < 1e36f)) s = amax >= 1e36f ? 0x1p-20f : 0x1p100f;
+  const float top = fmaxf(amax * s, 1e-30f), inv = rcp_approx(top);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float t = amax > 0.0f ? __fdiv_rn(127.0f * (v[e] * s), den) : 0.0f;
-    q[e] = (int)roundf(t);                                          // (NaN becomes 0)
+    const float a = 127.0f * fabsf(v[e] * s), on = __fadd_rd(a * inv, 8388608.0f);   // the quotient's floor on 2^23
+    const float half = (on - 8388608.0f) + 0.5f;
+    const int n = (__float_as_int(on) & 0xFF) + (fmaf(-half, top, a) >= 0.0f);       // (NaN: whatever, the scale is NaN)
+    q[e] = v[e] < 0.0f ? -n : n;
   }
-  return __fdiv_rn(amax, 127.0f);
+  return amax * 0.007874015748f;
 }
 
 __device__ __forceinline__ uint32_t moe_pack4(int a, int b, int c, int d) {
@@ -64,10 +74,28 @@ __device__ __forceinline__ float moe_act(int act, float g) {
   return act == GSQ_ACT_SILU ? __fdividef(g, 1.0f + expf(-g)) : 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
 }
 
+// A launch that may begin while the kernel before it in the stream still runs: it waits (griddepcontrol.wait) before it reads what that
+// kernel writes. What came before that kernel is over by then.
+template <typename K, typename... A>
+static int moe_launch_behind(K kern, unsigned blocks, unsigned threads, size_t smem, cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  GSQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, args...));
+  return GSQ_OK;
+}
+
 // gsq_moe_dot.cu: the two products for every pair, from xq / xd to h, from hq / hd to part
 int moe_dot_gate_up(const MoeArgs& a, int type, cudaStream_t st);
 int moe_dot_down(const MoeArgs& a, int type, cudaStream_t st);
-// gsq_moe_mma.cu: the same by groups, from x to h, from h to part
+// gsq_moe_mma.cu: the same by groups, from xq / xd to h, from h to part
 bool moe_mma_serves(int type, int k);
 int moe_mma_product(const MoeArgs& a, int type, bool down, cudaStream_t st);
 

@@ -3,15 +3,15 @@
 // The pairs of a token and one of its experts are gathered by expert, at most 8 to a group (gsq_moe.cu), so that an expert's
 // weights are read and decoded once for 8 tokens. A tile is 16 weight rows: 8 gate and the 8 up rows of the same channels, which
 // leaves a channel's gate and up sums in one lane, or 16 rows of the down weights. The list of (group, tile) is cut into one
-// contiguous range a block, one block an SM; a block takes as many groups of its range at a time as its columns of
+// contiguous range a block of equal estimated cost, one block an SM; a block takes as many groups of its range at a time as its columns of
 // activations hold (a batch, mostly all of them), and cuts the batch's superblocks into 16 equal contiguous chunks, one a warp.
 //
-//   * Weights: each warp has a ring of asynchronous copies of its own (16 rows x 1 superblock a stage, consecutive lanes on consecutive
-//     16-byte pieces of a row), filled ahead over tiles and batches, so the stream does not stop. Rows of 210- and 110-byte blocks start at any even address: copies begin at
+//   * Weights: each warp has a ring of asynchronous copies of its own (a stage is 16 rows x 2 superblocks, 1 for Q6_K; 16 lanes copy
+//     consecutive 16-byte pieces of a row), filled ahead over tiles and batches, so the stream does not stop. Rows of 210- and 110-byte blocks start at any even address: copies begin at
 //     the 16-byte boundary before, and the rows are read at their offset. (One bulk copy a row was a loop over the 16 lanes that
 //     issue them: 95 of 427 instructions a superblock.)
-//   * Activations: the block takes its batch's rows (X, or the activated products), quantises them into shared memory in the order of
-//     the tensor-core instruction's B fragment. An instruction takes the 8 columns from its group's first on; what it finds past the
+//   * Activations: the block takes its batch's rows (X in 8 bits, or the activated products, which it quantises) into shared memory in
+//     the order of the tensor-core instruction's B fragment. An instruction takes the 8 columns from its group's first on; what it finds past the
 //     group's own only reaches sums that are not stored.
 //   * Product: mma.sync m16n8k32 on bytes (m16n8k16 for Q6_K, whose sub-scales cover 16 values); a lane decodes exactly its share of
 //     the A fragment. Every sub-scale's sum has to be scaled on its own, and that, not the instruction, is the cost: with a column for
@@ -41,14 +41,15 @@ __device__ const uint32_t g_iq3s[512] = GSQ_IQ3S_GRID_INIT;
 __constant__ __align__(16) int8_t c_iq4[16] = GSQ_IQ4NL_VALUES_INIT;
 
 __host__ __device__ constexpr int bs(int kind) { return kind == Q4K ? 144 : kind == Q6K ? 210 : kind == IQ3S ? 110 : 136; }
+__host__ __device__ constexpr int stage_sb(int kind) { return kind == Q6K ? 1 : 2; }   // superblocks of a stage
 // Bytes between the rows of a stage: what a row's pieces may take (up to 14 bytes in front, 16-byte pieces), at distances that put what a
 // warp reads at once on different banks.
-__host__ __device__ constexpr int pitch(int kind) { return kind == Q4K ? 160 : kind == Q6K ? 240 : 144; }
+__host__ __device__ constexpr int pitch(int kind) { return kind == Q4K ? 288 : kind == Q6K ? 240 : kind == IQ3S ? 240 : 304; }
 constexpr int GRID_COPIES = 8;               // of IQ3_S's codebook in shared memory, one for lanes l, l + 8, ...
-constexpr int WINDOW = 64;                   // groups of a block that are looked up at a time
+constexpr int WINDOW = 32;                   // groups of a block that are looked up at a time
 __host__ __device__ constexpr size_t fixed_smem(int kind, int k, int cap) {   // all but the ring
   return (size_t)k * cap + (size_t)k / 32 * cap * 4 + (kind == Q4K ? (size_t)k / 256 * cap * 128 : 0) + (kind == IQ3S ? 512 * 4 * GRID_COPIES : 0) +
-         2 * WARPS * 512;
+         WARPS * 512;
 }
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -210,9 +211,12 @@ __device__ __forceinline__ void superblock(const uint8_t* b0, const uint8_t* b1,
   // raw words that several slices share
   uint2 q4[2];
   uint32_t l6[2][2][2], h6[2][2];
+  int half[4];
+  float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int f = 0; f < NC; ++f) {
-    int c[4] = {MAGIC, MAGIC, MAGIC, MAGIC};
+    constexpr int START = KIND == Q6K && TT == 8 ? 0 : MAGIC;
+    int c[4] = {START, START, START, START};
     uint2 fed_words = make_uint2(0, 0);
     if constexpr (KIND == Q6K) fed_words.x = x.quants16(f);
     else fed_words = x.quants(f);
@@ -283,6 +287,29 @@ __device__ __forceinline__ void superblock(const uint8_t* b0, const uint8_t* b1,
       }
     }
     const float2 d = x.scales(f);
+    if constexpr (KIND == Q6K && TT == 8) {
+      // halves of a slice: sum_a * scale_a + sum_b * scale_b as integers, converted once, scaled by d at the end
+      const int u0 = *reinterpret_cast<const int8_t*>(b0 + 192 + f), u1 = *reinterpret_cast<const int8_t*>(b1 + 192 + f);
+      const int n0 = u0 * c[0], n1 = u0 * c[1], n2 = u1 * c[2], n3 = u1 * c[3];
+      if (f & 1) {
+        part[0] = fmaf((float)(half[0] + n0), d.x, part[0]);
+        part[1] = fmaf((float)(half[1] + n1), d.y, part[1]);
+        part[2] = fmaf((float)(half[2] + n2), d.x, part[2]);
+        part[3] = fmaf((float)(half[3] + n3), d.y, part[3]);
+      } else {
+        half[0] = n0;
+        half[1] = n1;
+        half[2] = n2;
+        half[3] = n3;
+      }
+      if (f == NC - 1) {
+        acc[0] = fmaf(d0, part[0], acc[0]);
+        acc[1] = fmaf(d0, part[1], acc[1]);
+        acc[2] = fmaf(d1, part[2], acc[2]);
+        acc[3] = fmaf(d1, part[3], acc[3]);
+      }
+      continue;
+    }
     const float a00 = row_scale(0, f, 0), a10 = row_scale(1, f, 0), a01 = TT == 1 ? row_scale(0, f, 1) : a00, a11 = TT == 1 ? row_scale(1, f, 1) : a10;
     acc[0] = fmaf(fmaf(__int_as_float(c[0]), a00, -MAGIC_F * a00), d.x, acc[0]);
     acc[1] = fmaf(fmaf(__int_as_float(c[1]), a01, -MAGIC_F * a01), d.y, acc[1]);
@@ -333,33 +360,11 @@ __device__ __forceinline__ void fold(float (&acc)[4]) {
   }
 }
 
-// 8 consecutive activations of a row (piece `piece` of the row), in fp32.
-template <bool DOWN>
-__device__ __forceinline__ void load_act(const MoeArgs& a, int pair, int piece, float (&v)[8]) {
-  if constexpr (DOWN) {
-    load8<float, true>(a.h, (int64_t)pair * a.inter + 8 * piece, v);
-  } else {
-    const int64_t at = (int64_t)(pair / a.top_k) * a.x_stride + 8 * piece;
-    if (a.x_dtype == GSQ_F32) {
-      if (a.x_vec) load8<float, true>((const float*)a.x, at, v);
-      else load8<float, false>((const float*)a.x, at, v);
-    } else if (a.x_dtype == GSQ_F16) {
-      if (a.x_vec) load8<__half, true>((const __half*)a.x, at, v);
-      else load8<__half, false>((const __half*)a.x, at, v);
-    } else {
-      if (a.x_vec) load8<__nv_bfloat16, true>((const __nv_bfloat16*)a.x, at, v);
-      else load8<__nv_bfloat16, false>((const __nv_bfloat16*)a.x, at, v);
-    }
-  }
-}
-
-// 8 values of column `col` into the staged activations. Whole warps call it: four lanes share a slice of 32 values.
+// 8 quants of column `col` (words w0, w1; d: the scale of their 32, sum: the quants') into the staged activations. Whole warps call
+// it: four lanes share a slice of 32 values.
 template <int KIND, int CAP>
-__device__ __forceinline__ void stage_piece(const float (&v)[8], int piece, int col, int nsb, uint8_t* q_s, float* d_s, float* min_s) {
-  int q[8];
-  const float d = moe_quant8(v, q);
+__device__ __forceinline__ void stage_piece(uint32_t w0, uint32_t w1, float d, int piece, int col, int nsb, uint8_t* q_s, float* d_s, float* min_s) {
   const int s = piece >> 2, p = piece & 3;
-  const uint32_t w0 = moe_pack4(q[0], q[1], q[2], q[3]), w1 = moe_pack4(q[4], q[5], q[6], q[7]);
   uint8_t* to = q_s + (s * CAP + col) * 32;
   if constexpr (KIND == Q6K) {           // lane t's words t and 4 + t side by side
     *reinterpret_cast<uint32_t*>(to + 16 * (p & 1) + 4 * (p >> 1)) = w0;
@@ -372,10 +377,10 @@ __device__ __forceinline__ void stage_piece(const float (&v)[8], int piece, int 
     *reinterpret_cast<uint2*>(to + 8 * p) = make_uint2(w0, w1);
   }
   if constexpr (KIND == Q4K) {
-    int sum = q[0] + q[1] + q[2] + q[3] + q[4] + q[5] + q[6] + q[7];
+    int sum = dp4a((int)w0, 0x01010101, dp4a((int)w1, 0x01010101, 0));
     sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
     sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
-    if (p == 0) {                        // d * sum in three parts of at most 11 bits
+    if (p == 0) {                        // d * sum, and in three parts of at most 11 bits
       const float xs = d * (float)sum, hi = __uint_as_float(__float_as_uint(xs) & 0xFFFFE000u), r = xs - hi;
       const float mid = __uint_as_float(__float_as_uint(r) & 0xFFFFE000u);
       min_s[s * CAP + col] = xs;
@@ -386,6 +391,26 @@ __device__ __forceinline__ void stage_piece(const float (&v)[8], int piece, int 
     }
   }
   if (p == 0) d_s[s * CAP + col] = d;
+}
+
+// Stores a tile's sums: rows g, g + 8 by columns 2 t, 2 t + 1 of the group.
+template <bool DOWN>
+__device__ __forceinline__ void store_tile(const MoeArgs& a, const float (&acc)[4], int4 gr, int tile, const int* pair_s, const float* weight_s, int g, int t) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int col = 2 * t + c;
+    if (col < gr.z) {
+      const int pair = pair_s[gr.w + col];
+      if constexpr (DOWN) {
+        float* to = a.part + (int64_t)pair * a.hidden + 16 * tile + g;
+        const float wt = weight_s[gr.w + col];
+        to[0] = wt * acc[c];
+        to[8] = wt * acc[2 + c];
+      } else {
+        a.h[(int64_t)pair * a.inter + 8 * tile + g] = moe_act(a.act, acc[c]) * acc[2 + c];
+      }
+    }
+  }
 }
 
 // A batch: units (group, tile) [u0, u1) of the block's list; first of its groups in the window, and how many.
@@ -399,39 +424,37 @@ struct Window {
   int first, batches, end;   // number of the window's first group; one past its last unit
 };
 
-// Superblocks s0 .. s1 of a batch are warp `warp`'s.
-__device__ __forceinline__ int chunk_begin(const Batch& b, int nsb, int warp) { return (int)((int64_t)(b.u1 - b.u0) * nsb * warp / WARPS); }
+// A batch's steps (a stage's superblocks of a tile) from chunk_begin(warp) to chunk_begin(warp + 1) are warp `warp`'s. steps: of a tile.
+__device__ __forceinline__ int chunk_begin(const Batch& b, int steps, int warp) { return (b.u1 - b.u0) * steps * warp / WARPS; }
 
-// A warp's way through the superblocks of its chunks, batch after batch of a window.
+// A warp's way through the steps of its chunks, batch after batch of a window.
 struct Place {
-  int batch, s, s1;          // superblock of the batch, end of the chunk
-  int group, tile, sb;       // group of the window, tile of the group, superblock of the tile
+  int batch, left;           // steps left of the chunk
+  int group, tile, step;     // group of the window, tile of the group, step of the tile
   bool live;
-  __device__ __forceinline__ void enter(const Window& w, int tiles, int nsb, int warp) {   // `batch`, or the next one with work for this warp
+  __device__ __forceinline__ void enter(const Window& w, int tiles, int steps, int warp) {   // `batch`, or the next one with work for this warp
     for (live = false; !live && batch < w.batches; batch += !live) {
       const Batch b = w.batch[batch];
-      s = chunk_begin(b, nsb, warp);
-      s1 = chunk_begin(b, nsb, warp + 1);
-      if (s < s1) {
+      const int s = chunk_begin(b, steps, warp);
+      left = chunk_begin(b, steps, warp + 1) - s;
+      if (left > 0) {
         live = true;
-        const int u = s / nsb, at = b.u0 + u;
-        sb = s - u * nsb;
+        const int u = s / steps, at = b.u0 + u;
+        step = s - u * steps;
         group = at / tiles - w.first;
         tile = at - (group + w.first) * tiles;
       }
     }
   }
-  // the superblock behind; true where it is another tile's (or there is none left)
-  __device__ __forceinline__ bool next(const Window& w, int tiles, int nsb, int warp) {
-    ++s;
-    ++sb;
-    if (s == s1) {
+  // the step behind; true where it is another tile's (or there is none left)
+  __device__ __forceinline__ bool next(const Window& w, int tiles, int steps, int warp) {
+    if (--left == 0) {
       ++batch;
-      enter(w, tiles, nsb, warp);
+      enter(w, tiles, steps, warp);
       return true;
     }
-    if (sb < nsb) return false;
-    sb = 0;
+    if (++step < steps) return false;
+    step = 0;
     if (++tile == tiles) {
       tile = 0;
       ++group;
@@ -446,9 +469,11 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Window win;
   __shared__ int pair_s[CAP];
-  constexpr int PITCH = pitch(KIND), STAGE = 16 * PITCH, BS = bs(KIND);
+  __shared__ float weight_s[CAP];                    // (down product)
+  __shared__ int token_s[CAP];                       // (gate / up product)
+  constexpr int PITCH = pitch(KIND), STAGE = 16 * PITCH, BS = bs(KIND), SBS = stage_sb(KIND);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int k = DOWN ? a.inter : a.hidden, rows = DOWN ? a.hidden : 2 * a.inter, tiles = rows >> 4, nsb = k >> 8;
+  const int k = DOWN ? a.inter : a.hidden, rows = DOWN ? a.hidden : 2 * a.inter, tiles = rows >> 4, nsb = k >> 8, steps = (nsb + SBS - 1) / SBS;
   const int64_t rb = DOWN ? a.rb2 : a.rb13;
   const uint8_t* const weights = DOWN ? a.w2 : a.w13;
 
@@ -461,23 +486,28 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
   if (KIND == Q4K) sp += (size_t)k / 256 * CAP * 128;
   uint32_t* grid_s = reinterpret_cast<uint32_t*>(sp);
   if (KIND == IQ3S) sp += 512 * 4 * GRID_COPIES;
-  float4* part_s = reinterpret_cast<float4*>(sp);    // [warps][2][lanes]: sums of a tile that begins before the chunk, that ends behind it
-  sp += 2 * WARPS * 512;
+  float4* part_s = reinterpret_cast<float4*>(sp);    // [warps][lanes]: sums of the tile that begins before the warp's chunk
+  sp += WARPS * 512;
   const uint8_t* ring = sp + (size_t)warp * STAGES * STAGE;
-  // a stage's pieces: piece lane + 32 i of 16 rows of PIECES each. Their rows' offsets from row 0 and where they go do not change.
-  constexpr int PIECES = (BS + (KIND == Q4K ? 0 : KIND == IQ4XS ? 8 : 14) + 15) / 16, COPIES = (16 * PIECES + 31) / 32;
-  uint32_t from_row[COPIES], piece_at[COPIES];      // (offset of the piece's row from the tile's first; 16 * piece | slot offset << 8)
-#pragma unroll
-  for (int i = 0; i < COPIES; ++i) {
-    const int c = min(lane + 32 * i, 16 * PIECES - 1), r = c / PIECES, p = c - r * PIECES;
-    from_row[i] = (uint32_t)((DOWN ? r : (r & 7) + (r & 8 ? a.inter : 0)) * rb);
-    piece_at[i] = 16 * p | (r * PITCH + 16 * p) << 8;
-  }
-  const uint32_t copy_to = smem_addr(ring);
+  // copies of a stage: copy i has pieces lane % 16 of rows 2 i and 2 i + 1, and where a row has more than 16 pieces one copy takes
+  // pieces 16, 17 of all rows. Row r >= 8 of a gate / up tile is an up row.
+  constexpr int PIECES = (SBS * BS + (KIND == Q4K ? 0 : KIND == IQ4XS ? 8 : 14) + 15) / 16;
+  static_assert(PIECES <= 18 && 16 * PIECES <= PITCH, "");
+  const uint32_t to_rows = smem_addr(ring) + (lane >> 4) * PITCH + 16 * (lane & 15), to_rest = smem_addr(ring) + (lane >> 1) * PITCH + 256 + 16 * (lane & 1);
+  const int64_t up_rows = DOWN ? 0 : (a.inter - 8) * rb, from_rows = (lane >> 4) * rb, from_rest = (lane >> 1) * rb + (lane >= 16 ? up_rows : 0);
 
-  const int64_t units = (int64_t)*a.groups * tiles;
-  const int block_u1 = (int)(units * (blockIdx.x + 1) / gridDim.x);
-  int u0 = (int)(units * blockIdx.x / gridDim.x);
+  // Launched while the kernel before runs (launch_kernel). The gate / up product waits for the plan; the down product has the plan from
+  // before that product, and its first weights come in while that finishes.
+  if (!DOWN) asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // the block's units: boundary b is a group and a share (of 65536) of its tiles
+  auto boundary = [&](int b) {
+    const int2 at = a.bounds[b];
+    return at.x * tiles + (int)(((int64_t)at.y * tiles) >> 16);
+  };
+  const int block_u1 = boundary(blockIdx.x + 1);
+  int u0 = boundary(blockIdx.x);
   if (KIND == IQ3S)
     for (int i = tid; i < 512 * GRID_COPIES; i += THREADS) grid_s[i] = g_iq3s[i / GRID_COPIES];
 
@@ -513,26 +543,30 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
     // the weights' stream
     Place in;
     in.batch = 0;
-    in.enter(win, tiles, nsb, warp);
-    int64_t in_off = 0;                // of the tile's first row, at the next superblock
+    in.enter(win, tiles, steps, warp);
+    int64_t in_off = 0;                // of the tile's first row, at the next step
     auto row_offset = [&](const Place& p, int r) {
       const int row = DOWN ? 16 * p.tile + r : 8 * p.tile + (r & 7) + (r & 8 ? a.inter : 0);
-      return ((int64_t)win.group[p.group].x * rows + row) * rb + p.sb * BS;
+      return ((int64_t)win.group[p.group].x * rows + row) * rb + p.step * (SBS * BS);
     };
     if (in.live) in_off = row_offset(in, 0);
     auto issue = [&](int slot) {       // one stage's copies; an empty group of copies where there is nothing left
       if (in.live) {
+        const int bytes = (SBS == 2 && 2 * in.step + 1 == nsb ? 1 : SBS) * BS;   // (an odd row length: its last step is one superblock)
+        auto copy = [&](uint32_t to, int64_t row, int piece) {
+          const int front = KIND == Q4K ? 0 : (int)(row & 15);
+          if (16 * piece < front + bytes) copy16(to + slot * STAGE, weights + (row - front) + 16 * piece);
+        };
+        int64_t row = in_off + from_rows;
 #pragma unroll
-        for (int i = 0; i < COPIES; ++i) {
-          if (32 * i + 31 >= 16 * PIECES && lane + 32 * i >= 16 * PIECES) continue;
-          const uint32_t p = piece_at[i] & 255u;
-          const uint32_t to = copy_to + slot * STAGE + (piece_at[i] >> 8);
-          const int64_t off = in_off + from_row[i];
-          if (KIND == Q4K) copy16(to, weights + off + p);
-          else if (p < (uint32_t)(off & 15) + BS) copy16(to, weights + (off & ~(int64_t)15) + p);
+        for (int i = 0; i < 8; ++i) {
+          if (i == 4) row += up_rows;
+          copy(to_rows + 2 * i * PITCH, row, lane & 15);
+          row += 2 * rb;
         }
-        in_off += BS;
-        if (in.next(win, tiles, nsb, warp) && in.live) in_off = row_offset(in, 0);
+        if (PIECES > 16) copy(to_rest, in_off + from_rest, 16 + (lane & 1));
+        in_off += SBS * BS;
+        if (in.next(win, tiles, steps, warp) && in.live) in_off = row_offset(in, 0);
       }
       commit();
     };
@@ -541,63 +575,77 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
 
     Place at;
     at.batch = 0;
-    at.enter(win, tiles, nsb, warp);
+    at.enter(win, tiles, steps, warp);
     int slot = 0;
     for (int batch = 0; batch < win.batches; ++batch) {
       const Batch bt = win.batch[batch];
       {
         // columns of the batch: pairs, then their rows' values (unused columns in between hold what was there)
         __syncthreads();                // the batch before is done with them
+        if (DOWN) asm volatile("griddepcontrol.wait;" ::: "memory");
         if (tid < CAP) pair_s[tid] = -1;
         __syncthreads();
         if (tid < bt.n * 8) {
           const int4 gr = win.group[bt.g0 + (tid >> 3)];
-          if ((tid & 7) < gr.z) pair_s[gr.w + (tid & 7)] = a.list[gr.y + (tid & 7)];
+          if ((tid & 7) < gr.z) {
+            const int pair = a.list[gr.y + (tid & 7)];
+            pair_s[gr.w + (tid & 7)] = pair;
+            if (DOWN) weight_s[gr.w + (tid & 7)] = a.weights[pair];
+            else token_s[gr.w + (tid & 7)] = pair / a.top_k;
+          }
         }
         __syncthreads();
-        const int per = k >> 3, last = win.group[bt.g0 + bt.n - 1].w + win.group[bt.g0 + bt.n - 1].z, total = last * per;   // (whole warps: per % 32 == 0)
-        constexpr int U = 2;
-        for (int i0 = tid; i0 < total; i0 += U * THREADS) {
-          float v[U][8];
-          int pair[U];
+        // a warp takes a column's superblock at a time: 8 values a lane. X comes in quantised (by the blocks beside the plan's); the
+        // activated products are quantised here.
+        const int4 last = win.group[bt.g0 + bt.n - 1];
+        const int columns = last.w + last.z;
+        constexpr int U = 4;
+        int col = warp / nsb, sb = warp - col * nsb;
+        while (col < columns) {
+          uint4 raw[U][DOWN ? 2 : 1];
+          float d[U];
+          int at_col[U], at_sb[U];
 #pragma unroll
           for (int u = 0; u < U; ++u) {
-            const int i = i0 + u * THREADS;
-            pair[u] = i < total ? pair_s[i / per] : -1;
-            if (pair[u] >= 0) load_act<DOWN>(a, pair[u], i % per, v[u]);
+            const int row = col < columns ? pair_s[col] : -1;   // pair, or (gate / up) its token
+            at_col[u] = row >= 0 ? col : -1;
+            at_sb[u] = sb;
+            if (row >= 0) {
+              if constexpr (DOWN) {
+                const uint4* p = reinterpret_cast<const uint4*>(a.h + (int64_t)row * k + 256 * sb + 8 * lane);
+                raw[u][0] = __ldcg(p);
+                raw[u][DOWN] = __ldcg(p + 1);
+              } else {
+                const uint2 q = __ldcg(reinterpret_cast<const uint2*>(a.xq + (int64_t)token_s[col] * k + 256 * sb + 8 * lane));
+                raw[u][0] = make_uint4(q.x, q.y, 0, 0);
+                d[u] = __ldcg(a.xd + (int64_t)token_s[col] * (k >> 5) + 8 * sb + (lane >> 2));
+              }
+            }
+            for (sb += WARPS; sb >= nsb; sb -= nsb) ++col;
           }
 #pragma unroll
           for (int u = 0; u < U; ++u) {
-            const int i = i0 + u * THREADS;
-            if (pair[u] >= 0) stage_piece<KIND, CAP>(v[u], i % per, i / per, nsb, q_s, d_s, min_s);
+            if (at_col[u] < 0) continue;
+            uint32_t w0 = raw[u][0].x, w1 = raw[u][0].y;
+            if constexpr (DOWN) {
+              const float v[8] = {__uint_as_float(raw[u][0].x), __uint_as_float(raw[u][0].y), __uint_as_float(raw[u][0].z), __uint_as_float(raw[u][0].w),
+                                  __uint_as_float(raw[u][1].x), __uint_as_float(raw[u][1].y), __uint_as_float(raw[u][1].z), __uint_as_float(raw[u][1].w)};
+              int q[8];
+              d[u] = moe_quant8(v, q);
+              w0 = moe_pack4(q[0], q[1], q[2], q[3]);
+              w1 = moe_pack4(q[4], q[5], q[6], q[7]);
+            }
+            stage_piece<KIND, CAP>(w0, w1, d[u], 32 * at_sb[u] + lane, at_col[u], nsb, q_s, d_s, min_s);
           }
         }
         __syncthreads();
       }
-      // stores a tile's sums: rows g, g + 8 by columns 2 t, 2 t + 1 of the group
-      auto finish = [&](const float (&acc)[4], int group, int tile) {
-        const int4 gr = win.group[group];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int col = 2 * t + c;
-          if (col < gr.z) {
-            const int pair = pair_s[gr.w + col];
-            if constexpr (DOWN) {
-              float* to = a.part + (int64_t)pair * a.hidden + 16 * tile + g;
-              const float wt = a.weights[pair];
-              to[0] = wt * acc[c];
-              to[8] = wt * acc[2 + c];
-            } else {
-              a.h[(int64_t)pair * a.inter + 8 * tile + g] = moe_act(a.act, acc[c]) * acc[2 + c];
-            }
-          }
-        }
-      };
-      int open_unit = -1, open_group = 0, open_tile = 0;   // the tile that this warp has the beginning of, but not the end
+      int open_unit = -1;               // the tile that this warp has the beginning of, but not the end, and its sums so far
+      float open[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       while (at.live && at.batch == batch) {
         // a tile, or this warp's part of one
-        const int group = at.group, tile = at.tile, unit = bt.u0 + at.s / nsb;
-        const bool begins = at.sb == 0;
+        const int group = at.group, tile = at.tile, unit = (win.first + group) * tiles + tile;
+        const bool begins = at.step == 0;
         const int4 gr = win.group[group];
         float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         uint32_t p0 = 0, p1 = 0;        // a row begins in its stage at what its offset is past a 16-byte boundary
@@ -608,7 +656,7 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
         bool ends = false;
         auto run = [&](auto tokens) {
           constexpr int TT = decltype(tokens)::value;
-          Act<KIND, CAP, TT> x(q_s, d_s, min_s, nsb, at.sb, gr.w, g, t);
+          Act<KIND, CAP, TT> x(q_s, d_s, min_s, nsb, at.step * SBS, gr.w, g, t);
           bool more = true;
           do {
             wait_all_but<STAGES - 2>();
@@ -616,13 +664,19 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
             issue(slot == 0 ? STAGES - 1 : slot - 1);
             const uint8_t* b0 = ring + slot * STAGE + g * PITCH + (KIND == Q4K ? 0 : p0 & 15);
             const uint8_t* b1 = ring + slot * STAGE + (g + 8) * PITCH + (KIND == Q4K ? 0 : p1 & 15);
-            superblock<KIND, CAP, TT>(b0, b1, x, g, t, grid_s + (lane & (GRID_COPIES - 1)), acc);
-            x.next();
-            p0 += BS;
-            p1 += BS;
+            ends = at.step == steps - 1;
+            const int n = SBS == 2 && (!ends || (nsb & 1) == 0) ? 2 : 1;
+#pragma unroll 1                        // (one copy of the code: a kernel starts with none of it in the instruction cache)
+            for (int i = 0; i < n; ++i) {
+              superblock<KIND, CAP, TT>(b0, b1, x, g, t, grid_s + (lane & (GRID_COPIES - 1)), acc);
+              x.next();
+              b0 += BS;
+              b1 += BS;
+            }
+            p0 += SBS * BS;
+            p1 += SBS * BS;
             if (++slot == STAGES) slot = 0;
-            ends = at.sb == nsb - 1;
-            more = !at.next(win, tiles, nsb, warp);
+            more = !at.next(win, tiles, steps, warp);
           } while (more);
           fold<TT>(acc);
         };
@@ -631,30 +685,29 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
         else if (gr.z <= 4) run(std::integral_constant<int, 4>());
         else run(std::integral_constant<int, 8>());
         if (begins && ends) {
-          finish(acc, group, tile);
+          store_tile<DOWN>(a, acc, win.group[group], tile, pair_s, weight_s, g, t);
         } else {
-          part_s[(2 * warp + begins) * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
           if (begins) {
             open_unit = unit;
-            open_group = group;
-            open_tile = tile;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) open[i] = acc[i];
+          } else {
+            part_s[warp * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
           }
         }
       }
       __syncthreads();                  // all parts are there, and nobody reads the activations any more
       if (open_unit >= 0) {
-        const int tile_end = (open_unit - bt.u0 + 1) * nsb;
-        float4 v = part_s[(2 * warp + 1) * 32 + lane];
-        for (int o = warp + 1, from = chunk_begin(bt, nsb, o); from < tile_end; ++o) {
-          const int to = chunk_begin(bt, nsb, o + 1);
+        const int tile_end = (open_unit - bt.u0 + 1) * steps;
+        for (int o = warp + 1, from = chunk_begin(bt, steps, o); from < tile_end; ++o) {
+          const int to = chunk_begin(bt, steps, o + 1);
           if (to > from) {
-            const float4 q = part_s[2 * o * 32 + lane];
-            v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+            const float4 q = part_s[o * 32 + lane];
+            open[0] += q.x; open[1] += q.y; open[2] += q.z; open[3] += q.w;
           }
           from = to;
         }
-        const float acc[4] = {v.x, v.y, v.z, v.w};
-        finish(acc, open_group, open_tile);
+        store_tile<DOWN>(a, open, win.group[open_unit / tiles - win.first], open_unit % tiles, pair_s, weight_s, g, t);
       }
     }
   }
@@ -666,8 +719,8 @@ static int kind_of(int type) {
 
 // Columns of activations and stages of a warp's ring beside rows of k values. False: too long a row.
 static bool plan_of(int kind, int k, int max_smem, int* cap, int* stages, size_t* smem) {
-  const size_t room = (size_t)max_smem - 4096, stage = (size_t)WARPS * 16 * pitch(kind);   // (4096: the window and the driver's own)
-  const int plans[4][2] = {{16, 4}, {16, 3}, {8, 4}, {8, 2}};
+  const size_t room = (size_t)max_smem - 2304, stage = (size_t)WARPS * 16 * pitch(kind);   // (2304: the window, the columns and the driver's own)
+  const int plans[4][2] = {{16, 3}, {16, 2}, {8, 3}, {8, 2}};
   for (const auto& p : plans) {
     *cap = p[0];
     *stages = p[1];
@@ -680,9 +733,7 @@ static bool plan_of(int kind, int k, int max_smem, int* cap, int* stages, size_t
 template <int KIND, bool DOWN, int STAGES, int CAP>
 static int launch_kernel(const MoeArgs& a, size_t smem, int blocks, cudaStream_t st) {
   GSQ_CUDA_TRY(cudaFuncSetAttribute(moe_mma_kernel<KIND, DOWN, STAGES, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  moe_mma_kernel<KIND, DOWN, STAGES, CAP><<<blocks, THREADS, smem, st>>>(a);
-  GSQ_CUDA_TRY(cudaGetLastError());
-  return GSQ_OK;
+  return moe_launch_behind(moe_mma_kernel<KIND, DOWN, STAGES, CAP>, blocks, THREADS, smem, st, a);
 }
 
 template <int KIND, bool DOWN>
@@ -690,9 +741,9 @@ static int launch(const MoeArgs& a, const DeviceInfo& di, cudaStream_t st) {
   int cap, stages;
   size_t smem;
   if (!plan_of(KIND, DOWN ? a.inter : a.hidden, di.max_smem_optin, &cap, &stages, &smem)) return GSQ_ERR_UNSUPPORTED;
-  return cap == 16     ? (stages == 4 ? launch_kernel<KIND, DOWN, 4, 16>(a, smem, di.sm_count, st) : launch_kernel<KIND, DOWN, 3, 16>(a, smem, di.sm_count, st))
-         : stages == 4 ? launch_kernel<KIND, DOWN, 4, 8>(a, smem, di.sm_count, st)
-                       : launch_kernel<KIND, DOWN, 2, 8>(a, smem, di.sm_count, st);
+  const int blocks = di.sm_count < MOE_BLOCKS ? di.sm_count : MOE_BLOCKS;
+  if (cap == 16) return stages == 3 ? launch_kernel<KIND, DOWN, 3, 16>(a, smem, blocks, st) : launch_kernel<KIND, DOWN, 2, 16>(a, smem, blocks, st);
+  return stages == 3 ? launch_kernel<KIND, DOWN, 3, 8>(a, smem, blocks, st) : launch_kernel<KIND, DOWN, 2, 8>(a, smem, blocks, st);
 }
 
 }  // namespace moe
