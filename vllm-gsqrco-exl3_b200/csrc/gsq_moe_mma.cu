@@ -494,7 +494,8 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
   constexpr int PIECES = (SBS * BS + (KIND == Q4K ? 0 : KIND == IQ4XS ? 8 : 14) + 15) / 16;
   static_assert(PIECES <= 18 && 16 * PIECES <= PITCH, "");
   const uint32_t to_rows = smem_addr(ring) + (lane >> 4) * PITCH + 16 * (lane & 15), to_rest = smem_addr(ring) + (lane >> 1) * PITCH + 256 + 16 * (lane & 1);
-  const int64_t up_rows = DOWN ? 0 : (a.inter - 8) * rb, from_rows = (lane >> 4) * rb, from_rest = (lane >> 1) * rb + (lane >= 16 ? up_rows : 0);
+  const uint8_t* const from_piece = weights + 16 * (lane & 15);
+  const int64_t two_rows = 2 * rb, up_rows = DOWN ? 0 : (a.inter - 8) * rb, from_rows = (lane >> 4) * rb, from_rest = (lane >> 1) * rb + (lane >= 16 ? up_rows : 0);
 
   // Launched while the kernel before runs (launch_kernel). The gate / up product waits for the plan; the down product has the plan from
   // before that product, and its first weights come in while that finishes.
@@ -552,19 +553,33 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
     if (in.live) in_off = row_offset(in, 0);
     auto issue = [&](int slot) {       // one stage's copies; an empty group of copies where there is nothing left
       if (in.live) {
-        const int bytes = (SBS == 2 && 2 * in.step + 1 == nsb ? 1 : SBS) * BS;   // (an odd row length: its last step is one superblock)
-        auto copy = [&](uint32_t to, int64_t row, int piece) {
-          const int front = KIND == Q4K ? 0 : (int)(row & 15);
-          if (16 * piece < front + bytes) copy16(to + slot * STAGE, weights + (row - front) + 16 * piece);
+        const bool half = SBS == 2 && 2 * in.step + 1 == nsb;      // (an odd row length: its last step is one superblock)
+        const int bytes = half ? BS : SBS * BS;
+        // pieces 0 .. 15 of rows of two superblocks of 136 or 144 bytes, and 0 .. 13 of 210 bytes, are always needed
+        constexpr bool ALL = KIND == Q4K || KIND == IQ4XS || KIND == Q6K;
+        const bool mine = KIND != Q6K || (lane & 15) < 14;
+        auto copy = [&](uint32_t to, const uint8_t* from, int64_t row, int piece, bool sure) {
+          if (sure || 16 * piece < (KIND == Q4K ? 0 : (int)(row & 15)) + bytes) copy16(to + slot * STAGE, from + (KIND == Q4K ? row : row & ~(int64_t)15));
         };
         int64_t row = in_off + from_rows;
+        if (ALL && !half) {
+          if (mine) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (i == 4) row += up_rows;
-          copy(to_rows + 2 * i * PITCH, row, lane & 15);
-          row += 2 * rb;
+            for (int i = 0; i < 8; ++i) {
+              if (i == 4) row += up_rows;
+              copy(to_rows + 2 * i * PITCH, from_piece, row, 0, true);
+              row += two_rows;
+            }
+          }
+        } else {
+#pragma unroll 2
+          for (int i = 0; i < 8; ++i) {
+            if (i == 4) row += up_rows;
+            copy(to_rows + 2 * i * PITCH, from_piece, row, lane & 15, false);
+            row += two_rows;
+          }
         }
-        if (PIECES > 16) copy(to_rest, in_off + from_rest, 16 + (lane & 1));
+        if (PIECES > 16) copy(to_rest, weights + 256 + 16 * (lane & 1), in_off + from_rest, 16 + (lane & 1), false);
         in_off += SBS * BS;
         if (in.next(win, tiles, steps, warp) && in.live) in_off = row_offset(in, 0);
       }
