@@ -33,11 +33,9 @@ struct RouteArgs {
   int32_t* ids;
 };
 
-// One warp, one token; lane l holds experts l, l + 32, ... Each round takes the largest key, the lowest number among equals.
+// Scores and keys of a token, one warp: lane l holds experts l, l + 32, ...
 template <int PER_LANE>
-__device__ __forceinline__ void route_token(const RouteArgs& a, int token, int lane) {
-  float s[PER_LANE];
-  uint32_t key[PER_LANE];
+__device__ __forceinline__ void route_scores(const RouteArgs& a, int token, int lane, float (&s)[PER_LANE], uint32_t (&key)[PER_LANE]) {
   float top = -INFINITY;
   // (one branch on the type around all loads: they are under way together)
   const int64_t row = token * a.stride;
@@ -86,35 +84,70 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int token, int l
     for (int i = 0; i < PER_LANE; ++i)
       if (key[i]) key[i] = score_key(s[i] + a.bias[lane + 32 * i]);
   }
-  float mine = 0.0f, total = 0.0f;   // lane r keeps round r's choice
-  int id = -1;
-  for (int r = 0; r < a.top_k; ++r) {
-    uint32_t k = 0;
-    int at = 0;
+}
+
+// One warp, one token. Each lane puts its experts in order (larger key first, lower number first among equals); each round takes the
+// largest of the lanes' first ones, the lowest number among equals, and its lane goes on to its next.
+template <int PER_LANE>
+__device__ __forceinline__ void route_token(const RouteArgs& a, int token, int lane) {
+  float s[PER_LANE];
+  uint32_t key[PER_LANE];
+  route_scores<PER_LANE>(a, token, lane, s, key);
+  uint32_t first[PER_LANE];
+  int at[PER_LANE];
 #pragma unroll
-    for (int i = 0; i < PER_LANE; ++i)
-      if (key[i] > k) {
-        k = key[i];
-        at = i;
-      }
-    const uint32_t best = __reduce_max_sync(0xFFFFFFFFu, k);
-    if (best == 0) break;
-    const uint32_t e = __reduce_min_sync(0xFFFFFFFFu, k == best ? (uint32_t)(lane + 32 * at) : 0xFFFFFFFFu);
-    float w = 0.0f;
-    const bool owner = (e & 31) == (uint32_t)lane;
-#pragma unroll
-    for (int i = 0; i < PER_LANE; ++i)
-      if (owner && i == (int)(e >> 5)) {
-        w = s[i];
-        key[i] = 0;
-      }
-    w = __shfl_sync(0xFFFFFFFFu, w, e & 31);
-    total += w;
-    if (lane == r) {
-      mine = w;
-      id = (int)e;
-    }
+  for (int i = 0; i < PER_LANE; ++i) {
+    first[i] = key[i];
+    at[i] = i;
   }
+  if constexpr (PER_LANE <= 8) {
+#pragma unroll
+    for (int i = 1; i < PER_LANE; ++i)
+#pragma unroll
+      for (int j = i; j > 0; --j)
+        if (first[j] > first[j - 1]) {             // (insertion: equal ones stay in order)
+          const uint32_t k = first[j];
+          first[j] = first[j - 1];
+          first[j - 1] = k;
+          const int n = at[j];
+          at[j] = at[j - 1];
+          at[j - 1] = n;
+        }
+  }
+  int id = -1;                                     // lane r keeps round r's choice
+  for (int r = 0; r < a.top_k; ++r) {
+    if constexpr (PER_LANE > 8) {                  // (too many to put in order: the largest left to the front each time)
+#pragma unroll
+      for (int i = PER_LANE - 1; i > 0; --i)
+        if (first[i] > first[i - 1] || (first[i] == first[i - 1] && at[i] < at[i - 1])) {
+          const uint32_t k = first[i];
+          first[i] = first[i - 1];
+          first[i - 1] = k;
+          const int n = at[i];
+          at[i] = at[i - 1];
+          at[i - 1] = n;
+        }
+    }
+    const uint32_t best = __reduce_max_sync(0xFFFFFFFFu, first[0]);
+    if (best == 0) break;
+    const uint32_t e = __reduce_min_sync(0xFFFFFFFFu, first[0] == best ? (uint32_t)(lane + 32 * at[0]) : 0xFFFFFFFFu);
+    if ((e & 31) == (uint32_t)lane) {
+#pragma unroll
+      for (int i = 1; i < PER_LANE; ++i) {
+        first[i - 1] = first[i];
+        at[i - 1] = at[i];
+      }
+      first[PER_LANE - 1] = 0;
+    }
+    if (lane == r) id = (int)e;
+  }
+  float mine = 0.0f, total = 0.0f;
+#pragma unroll
+  for (int i = 0; i < PER_LANE; ++i) {
+    const float v = __shfl_sync(0xFFFFFFFFu, s[i], id & 31);
+    if (id >= 0 && (id >> 5) == i) mine = v;
+  }
+  for (int r = 0; r < a.top_k; ++r) total += __shfl_sync(0xFFFFFFFFu, mine, r);
   if (lane < a.top_k) {
     if (a.renormalize) mine = total > 0.0f ? __fdiv_rn(mine, total) : 0.0f;
     a.weights[(int64_t)token * a.top_k + lane] = mine * a.scale;
@@ -174,18 +207,27 @@ static int launch_quant(const void* x, int dtype, int vec, int64_t stride, int64
 }
 
 // y = sum of a token's parts, in the order of its choices.
-__global__ void __launch_bounds__(256) moe_combine_kernel(const MoeArgs a) {
+constexpr int COMBINE_THREADS = 64;               // (a token's 2048 values on 8 SMs)
+__global__ void __launch_bounds__(COMBINE_THREADS) moe_combine_kernel(const MoeArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int per_row = a.hidden >> 2;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, t = i / per_row;
+  const int64_t i = (int64_t)blockIdx.x * COMBINE_THREADS + threadIdx.x, t = i / per_row;
   if (t >= a.m) return;
   const int c = 4 * (int)(i - t * per_row);
   float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int r = 0; r < a.top_k; ++r) {
-    const int64_t pair = t * a.top_k + r;
-    if (moe_expert(a, (int)pair) < 0) continue;
-    const float4 p = *reinterpret_cast<const float4*>(a.part + pair * a.hidden + c);
-    s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
+  constexpr int U = 8;                            // parts under way together
+  for (int r0 = 0; r0 < a.top_k; r0 += U) {
+    bool here[U];
+    float4 p[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) here[u] = r0 + u < a.top_k && moe_expert(a, (int)(t * a.top_k) + r0 + u) >= 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) p[u] = here[u] ? __ldcg(reinterpret_cast<const float4*>(a.part + (t * a.top_k + r0 + u) * a.hidden + c)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (here[u]) {
+        s.x += p[u].x; s.y += p[u].y; s.z += p[u].z; s.w += p[u].w;
+      }
   }
   const int64_t at = t * a.y_stride + c;
   store_out_dyn(a.y, a.x_dtype, at, s.x);
@@ -465,7 +507,7 @@ static int run_experts(const gsq_moe* w, const void* x, int x_dtype, int64_t m, 
       if (rc == GSQ_OK) rc = moe_dot_down(a, w->w2_type, st);
     }
     if (rc != GSQ_OK) return rc;
-    rc = moe_launch_behind(moe_combine_kernel, (unsigned)(((int64_t)a.m * (a.hidden >> 2) + 255) / 256), 256, 0, st, a);
+    rc = moe_launch_behind(moe_combine_kernel, (unsigned)(((int64_t)a.m * (a.hidden >> 2) + COMBINE_THREADS - 1) / COMBINE_THREADS), COMBINE_THREADS, 0, st, a);
     if (rc != GSQ_OK) return rc;
   }
   return GSQ_OK;

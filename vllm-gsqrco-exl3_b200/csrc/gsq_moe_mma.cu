@@ -726,6 +726,7 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
       }
     }
   }
+  if (DOWN) asm volatile("griddepcontrol.wait;" ::: "memory");   // (blocks without work, too: what comes next may reuse the workspace)
 }
 
 static int kind_of(int type) {
