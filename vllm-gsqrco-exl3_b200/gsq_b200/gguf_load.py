@@ -9,11 +9,16 @@ on the device, and the IQ3_S / Q6_K runs are repacked in place by the CUDA repac
 (process_weights_after_loading -> gsq_iq3s_repack / gsq_q6k_repack). `unpack` still returns GGUF bytes for a consumer
 that needs them.
 
-Only what the linear path needs is here: tensor enumeration and fused-layer construction. Model architecture,
-tokenizer and config handling of the reference's loader are not.
+A mixture-of-experts layer's stacks ([experts, rows, row bytes] in the file) are read the same way into the two tensors that
+quantization.fused_moe takes; they stay in GGUF order.
+
+Only what these layers need is here: tensor enumeration and layer construction. Model architecture, tokenizer and config
+handling of the reference's loader are not.
 """
 
 from __future__ import annotations
+
+import contextlib
 
 import numpy as np
 import torch
@@ -114,3 +119,41 @@ def load_linear(path_or_tensors, names: list[str], device="cuda:0", params_dtype
         method.process_weights_after_loading(layer)          # pads, places, repacks IQ3_S / Q6_K runs on the GPU
         torch.cuda.synchronize()
     return layer, method
+
+
+def load_experts(path_or_tensors, gate: str, up: str, down: str, device="cuda:0", experts: slice | None = None, stager: _Stager | None = None):
+    """The experts of one layer from the named stacks of a GGUF file ([experts, inter, hidden] gate and up, [experts, hidden,
+    inter] down): -> (w13, w2, w13_type, w2_type) for fused_moe.moe_layer_gguf / fused_moe_gguf. `experts` (step 1) takes a
+    range of them: an expert-parallel rank's share, which fused_moe_gguf numbers from 0. Gate and up rows of an expert follow each other,
+    so the two must have one type."""
+    tens = tensors(path_or_tensors) if isinstance(path_or_tensors, str) else path_or_tensors
+    names = (gate, up, down)
+    for n in names:
+        if tens[n][0] not in ops.LCPP_QUANT_TYPES or tens[n][1].ndim != 3:
+            raise ValueError(f"load_experts: {n} is not a stack of quantised matrices of a served type")
+    (t13, g), (tu, u), (t2, d) = (tens[n] for n in names)
+    if t13 != tu or g.shape != u.shape:
+        raise ValueError(f"load_experts: {gate} and {up} differ in type or shape: {t13} {g.shape}, {tu} {u.shape}")
+    inter = d.shape[2] // ops.GGML_QUANT_SIZES[t2][1] * ops.GGML_QUANT_SIZES[t2][0]
+    hidden = g.shape[2] // ops.GGML_QUANT_SIZES[t13][1] * ops.GGML_QUANT_SIZES[t13][0]
+    if d.shape[:2] != (g.shape[0], hidden) or g.shape[1] != inter:
+        raise ValueError(f"load_experts: {down} {d.shape} does not fit {gate} {g.shape}: {hidden} rows of {g.shape[1]} values expected")
+    first, last, step = (experts or slice(None)).indices(g.shape[0])
+    if step != 1 or last <= first:
+        raise ValueError(f"load_experts: experts={experts} takes none of {g.shape[0]} or leaves gaps")
+    n = last - first
+    cuda = torch.device(device).type == "cuda"
+    with torch.cuda.device(device) if cuda else contextlib.nullcontext():
+        stager = stager or _Stager(device)
+        w13 = torch.empty((n, 2 * inter, g.shape[2]), dtype=torch.uint8, device=device)
+        w2 = torch.empty((n, *d.shape[1:]), dtype=torch.uint8, device=device)
+        for src, dst in ((g, w13[:, :inter]), (u, w13[:, inter:]), (d, w2)):
+            src, size = src[first:last], dst[0].numel()
+            if size <= _CHUNK:                                 # several experts to a chunk: an expert is one row of the copy
+                stager.to_device(src.reshape(n, size), dst.as_strided((n, size), (dst.stride(0), 1)))
+            else:
+                for e in range(n):
+                    stager.to_device(src[e], dst[e])
+        if cuda:
+            torch.cuda.synchronize()
+    return w13, w2, t13, t2
