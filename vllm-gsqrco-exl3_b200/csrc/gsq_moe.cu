@@ -236,11 +236,13 @@ __global__ void __launch_bounds__(COMBINE_THREADS) moe_combine_kernel(const MoeA
   store_out_dyn(a.y, a.x_dtype, at + 3, s.w);
 }
 
-// What a tile of the groups of n pairs costs, in 16ths of one of a single token: as measured on groups of 1, 2, 4 and 8 (Q4_K 174, 190,
-// 193, 220 us for one layer; the other types differ less).
-__device__ __forceinline__ int moe_cost(int n) {
-  const int r = n & 7;
-  return (n >> 3) * 20 + (r == 0 ? 0 : r == 1 ? 16 : r == 2 ? 17 : r <= 4 ? 18 : 20);
+// What a tile of the groups of n pairs costs, in 256ths of one of a single token (in 16ths, the blocks' shares of few experts were as coarse as a
+// share): as measured on groups of 1, 2, 4 and 8 (Q4_K 174, 190,
+// 193, 220 us for one layer; the other types differ less) and of 16 (1.4 times 8; the others 1.2).
+constexpr int COST_8 = 320, COST_16 = 416;
+__device__ __forceinline__ int moe_cost(int n, int group_max) {
+  const int r = n & (group_max - 1);
+  return (group_max == 8 ? (n >> 3) * COST_8 : (n >> 4) * COST_16) + (r == 0 ? 0 : r == 1 ? 256 : r == 2 ? 272 : r <= 4 ? 288 : r <= 8 ? COST_8 : COST_16);
 }
 
 // Pairs by expert: group, list, bounds. Block 0; PER_LANE > 0: it makes the choice first (few tokens). An expert's pairs stay in
@@ -256,7 +258,6 @@ __global__ void __launch_bounds__(PLAN_THREADS) moe_plan_kernel(const MoeArgs a,
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, pairs = a.m * a.top_k, experts = a.experts;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (blockIdx.x > 0) {                                          // the other blocks quantise X meanwhile
-
     const int64_t i = (int64_t)(blockIdx.x - 1) * PLAN_THREADS + tid;
     if (a.x_dtype == GSQ_F32) {
       if (a.x_vec) quant_piece<float, true>(a.x, a.x_stride, a.m, a.hidden, a.xq, a.xd, i);
@@ -301,7 +302,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) moe_plan_kernel(const MoeArgs a,
     __syncthreads();
   }
   // sums over the experts before: pairs, groups, cost
-  const int g = (n + 7) >> 3, cost = moe_cost(n);
+  const int most = a.group_max, g = (n + most - 1) >> (most == 8 ? 3 : 4), cost = moe_cost(n, most);
   int3 upto = make_int3(n, g, cost);
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -323,24 +324,24 @@ __global__ void __launch_bounds__(PLAN_THREADS) moe_plan_kernel(const MoeArgs a,
   place[tid] = upto.x - n;
   cost_upto[tid] = upto.z;
   group_upto[tid] = upto.y;
-  for (int i = 0; i < g; ++i) a.group[upto.y - g + i] = make_int4(tid, upto.x - n + 8 * i, min(8, n - 8 * i), 0);
+  for (int i = 0; i < g; ++i) a.group[upto.y - g + i] = make_int4(tid, upto.x - n + most * i, min(most, n - most * i), 0);
   __syncthreads();
 
   // block b of the products begins at cost total * b / blocks: in the first expert whose groups end behind that
   for (int b = tid; b <= a.blocks; b += PLAN_THREADS) {
     int2 at = make_int2(groups, 0);
     if (b < a.blocks && total > 0) {
-      const int target = (int)((uint32_t)total * b / a.blocks);   // (below 32768 * 16 * 256 = 2^27)
+      const int target = (int)((uint32_t)total * b / a.blocks);   // (total: at most 32768 * 256 = 2^23, b up to 2^8)
       int lo = 0, hi = experts - 1;
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
         if (cost_upto[mid] > target) hi = mid;
         else lo = mid + 1;
       }
-      // its groups: full ones of moe_cost(8), then the rest
-      const int first = lo ? group_upto[lo - 1] : 0, in = target - (lo ? cost_upto[lo - 1] : 0);
-      const int i = min(in / moe_cost(8), group_upto[lo] - first - 1), rest = in - i * moe_cost(8);
-      const int whole = min(moe_cost(8), cost_upto[lo] - (lo ? cost_upto[lo - 1] : 0) - i * moe_cost(8));
+      // its groups: full ones, then the rest
+      const int full = most == 8 ? COST_8 : COST_16, first = lo ? group_upto[lo - 1] : 0, before = lo ? cost_upto[lo - 1] : 0, in = target - before;
+      const int i = min(in / full, group_upto[lo] - first - 1), rest = in - i * full;
+      const int whole = min(full, cost_upto[lo] - before - i * full);
       at = make_int2(first + i, (rest << 16) / whole);
     }
     a.bounds[b] = at;
@@ -480,7 +481,9 @@ static int run_experts(const gsq_moe* w, const void* x, int x_dtype, int64_t m, 
   a.hq = (int8_t*)(ws + l.hq);
   a.hd = (float*)(ws + l.hd);
   a.part = (float*)(ws + l.part);
-  const bool up_mma = moe_mma_serves(w->w13_type, a.hidden), down_mma = moe_mma_serves(w->w2_type, a.inter);
+  a.many = m * top_k > 4 * w->experts;
+  const int up_mma = moe_mma_serves(w->w13_type, a.hidden, a.many), down_mma = moe_mma_serves(w->w2_type, a.inter, a.many);
+  a.group_max = up_mma == 8 || down_mma == 8 ? 8 : 16;
   for (int64_t t0 = 0; t0 < m; t0 += PASS_TOKENS) {
     a.m = (int)(m - t0 < PASS_TOKENS ? m - t0 : PASS_TOKENS);
     a.x = (const uint8_t*)x + t0 * x_row_stride * es;

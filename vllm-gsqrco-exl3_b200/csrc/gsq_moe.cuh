@@ -27,7 +27,9 @@ struct MoeArgs {
   float *xd, *hd;              // their scales, one per 32 values
   float* h;                    // [pairs][inter]: act(gate) * up
   float* part;                 // [pairs][hidden]: weight times down product
-  // pairs by expert, at most 8 to a group
+  // pairs by expert, at most group_max (8 or 16) to a group
+  int group_max;
+  bool many;                   // pairs: more than 4 an expert on average
   int2* bounds;                // [blocks + 1]: where a block's share of (group, tile) begins: a group, and 65536ths of its tiles
   int blocks;                  // of the products
   int4* group;                 // expert, first place in the list, pairs
@@ -96,7 +98,7 @@ static int moe_launch_behind(K kern, unsigned blocks, unsigned threads, size_t s
 int moe_dot_gate_up(const MoeArgs& a, int type, cudaStream_t st);
 int moe_dot_down(const MoeArgs& a, int type, cudaStream_t st);
 // gsq_moe_mma.cu: the same by groups, from xq / xd to h, from h to part
-bool moe_mma_serves(int type, int k);
+int moe_mma_serves(int type, int k, bool many);
 int moe_mma_product(const MoeArgs& a, int type, bool down, cudaStream_t st);
 
 }  // namespace gsq

@@ -41,15 +41,21 @@ __device__ const uint32_t g_iq3s[512] = GSQ_IQ3S_GRID_INIT;
 __constant__ __align__(16) int8_t c_iq4[16] = GSQ_IQ4NL_VALUES_INIT;
 
 __host__ __device__ constexpr int bs(int kind) { return kind == Q4K ? 144 : kind == Q6K ? 210 : kind == IQ3S ? 110 : 136; }
-__host__ __device__ constexpr int stage_sb(int kind) { return kind == Q6K ? 1 : 2; }   // superblocks of a stage
 // Bytes between the rows of a stage: what a row's pieces may take (up to 14 bytes in front, 16-byte pieces), at distances that put what a
 // warp reads at once on different banks.
-__host__ __device__ constexpr int pitch(int kind) { return kind == Q4K ? 288 : kind == Q6K ? 240 : kind == IQ3S ? 240 : 304; }
+__host__ __device__ constexpr int pitch(int kind, int sbs) {
+  return kind == Q6K ? 240 : sbs == 1 ? 144 : kind == Q4K ? 288 : kind == IQ3S ? 240 : 304;
+}
+// Where row r of 16 is in a stage. Q4_K's 8-byte reads take rows 0 .. 3, then 4 .. 7 at once: at 144 bytes a row these have to be every
+// second one.
+template <int KIND, int SBS>
+__host__ __device__ constexpr int row_place(int r) {
+  return KIND == Q4K && SBS == 1 ? (r & 8) | (r & 3) << 1 | (r >> 2 & 1) : r;
+}
 constexpr int GRID_COPIES = 8;               // of IQ3_S's codebook in shared memory, one for lanes l, l + 8, ...
 constexpr int WINDOW = 32;                   // groups of a block that are looked up at a time
 __host__ __device__ constexpr size_t fixed_smem(int kind, int k, int cap) {   // all but the ring
-  return (size_t)k * cap + (size_t)k / 32 * cap * 4 + (kind == Q4K ? (size_t)k / 256 * cap * 128 : 0) + (kind == IQ3S ? 512 * 4 * GRID_COPIES : 0) +
-         WARPS * 512;
+  return (size_t)k * cap + (size_t)k / 32 * cap * 4 * (kind == Q4K ? 2 : 1) + (kind == IQ3S ? 512 * 4 * GRID_COPIES : 0) + WARPS * 64 * cap;
 }
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -94,7 +100,7 @@ __device__ __forceinline__ uint32_t lds16(const uint8_t* p) { return *reinterpre
 __device__ __forceinline__ uint32_t lds32(const uint8_t* p) { return *reinterpret_cast<const uint32_t*>(p); }
 __device__ __forceinline__ uint32_t lds32h(const uint8_t* p) { return prmt(lds16(p), lds16(p + 2), 0x5410); }   // from an even address
 
-// How a group of up to TT tokens uses the 8 columns of a C fragment: NJ parts (slices of 32 values; of 16 for Q6_K) times TT tokens,
+// How a group of up to TT tokens (16: twice 8) uses the 8 columns of a C fragment: NJ parts (slices of 32 values; of 16 for Q6_K) times TT tokens,
 // column j TT + token. A superblock is NC fragments. Lane (g, t) feeds column g, and has the sums of columns 2 t, 2 t + 1.
 template <int KIND, int TT>
 struct Columns {
@@ -107,38 +113,39 @@ struct Columns {
 // What a lane reads of the staged activations of one superblock, CAP columns a slice.
 template <int KIND, int CAP, int TT>
 struct Act {
-  using Col = Columns<KIND, TT>;
+  static constexpr int TF = TT < 8 ? TT : 8;   // tokens of a fragment; of 16, fragment n has columns 8 n ..
+  using Col = Columns<KIND, TF>;
   const uint8_t* q;        // [slice][column][32 bytes]
   const float* d;          // [slice][column]
-  const float* sums;       // [slice][column]: d * sum of the quants (Q4_K)
-  const float* mins;       // the same in parts, [part][column][t][2]
+  const float* sums;       // [slice][column]: d * sum of the quants (Q4_K); of column 2 t
+  const float* mins;       // the same of slice t, column g
   // col: the group's first column
-  __device__ __forceinline__ Act(const uint8_t* q_s, const float* d_s, const float* min_s, int nsb, int sb, int col, int g, int t) {
+  __device__ __forceinline__ Act(const uint8_t* q_s, const float* d_s, const float* sum_s, int sb, int col, int g, int t) {
     const int j = Col::fed_part(g), i = Col::part(t, 0), s = KIND == Q6K ? i >> 1 : i;
     q = q_s + ((sb * 8 + (KIND == Q6K ? j >> 1 : j)) * CAP + col + Col::fed_token(g)) * 32 + 8 * t + (KIND == Q6K ? 4 * (j & 1) : 0);
-    d = d_s + (sb * 8 + s) * CAP + col + 2 * t % TT;
-    sums = min_s + (sb * 8 + s) * CAP + col + 2 * t % TT;
-    mins = min_s + nsb * 8 * CAP + sb * (CAP * 24) + ((col + g) * 4 + t) * 2;
+    d = d_s + (sb * 8 + s) * CAP + col + 2 * t % TF;
+    sums = sum_s + (sb * 8 + s) * CAP + col + 2 * t % TF;
+    mins = sum_s + (sb * 8 + t) * CAP + col + g;
   }
   __device__ __forceinline__ void next() {
     q += CAP * 256;
     d += CAP * 8;
     sums += CAP * 8;
-    mins += CAP * 24;
+    mins += CAP * 8;
   }
-  // this lane's words of the part that it feeds in fragment c
-  __device__ __forceinline__ uint2 quants(int c) const { return *reinterpret_cast<const uint2*>(q + CAP * 32 * Col::NJ * c); }
-  __device__ __forceinline__ uint32_t quants16(int c) const {
-    return *reinterpret_cast<const uint32_t*>(q + (TT == 8 ? CAP * 32 * (c >> 1) + 4 * (c & 1) : CAP * 16 * Col::NJ * c));
+  // this lane's words of the part that it feeds in fragment c (of the columns from 8 n on)
+  __device__ __forceinline__ uint2 quants(int c, int n) const { return *reinterpret_cast<const uint2*>(q + CAP * 32 * Col::NJ * c + 256 * n); }
+  __device__ __forceinline__ uint32_t quants16(int c, int n) const {
+    return *reinterpret_cast<const uint32_t*>(q + (TF == 8 ? CAP * 32 * (c >> 1) + 4 * (c & 1) : CAP * 16 * Col::NJ * c) + 256 * n);
   }
   static __device__ __forceinline__ float2 two(const float* p, int c) {
-    const int s = KIND != Q6K ? Col::NJ * c : TT == 8 ? c >> 1 : Col::NJ / 2 * c;
-    if constexpr (TT > 1) return *reinterpret_cast<const float2*>(p + CAP * s);
+    const int s = KIND != Q6K ? Col::NJ * c : TF == 8 ? c >> 1 : Col::NJ / 2 * c;
+    if constexpr (TF > 1) return *reinterpret_cast<const float2*>(p + CAP * s);
     return make_float2(p[CAP * s], p[CAP * (s + (KIND != Q6K))]);   // (Q6_K: two halves of a slice)
   }
-  __device__ __forceinline__ float2 scales(int c) const { return two(d, c); }
+  __device__ __forceinline__ float2 scales(int c, int n) const { return two(d + 8 * n, c); }
   __device__ __forceinline__ float2 quant_sums(int c) const { return two(sums, c); }
-  __device__ __forceinline__ float2 minima(int part) const { return *reinterpret_cast<const float2*>(mins + CAP * 8 * part); }
+  __device__ __forceinline__ float2 minima(int n) const { return make_float2(mins[8 * n], mins[CAP * 4 + 8 * n]); }   // slices t, t + 4
 };
 
 // Byte `at` (of 8 in two words) as a number on 2^23.
@@ -146,11 +153,13 @@ __device__ __forceinline__ float byte_on_2_23(const uint32_t (&w)[2], bool upper
   return __uint_as_float(prmt(upper ? w[1] : w[0], 0x4B000000u, 0x7440u | at));
 }
 
-// One superblock of 16 rows: b0, b1 = the blocks of rows g and g + 8; acc: rows g, g + 8 by columns 2 t, 2 t + 1 of the C fragments.
+// One superblock of 16 rows: b0, b1 = the blocks of rows g and g + 8; acc: rows g, g + 8 by columns 2 t, 2 t + 1 of the C fragments (of the
+// first 8 columns, then of the others).
 template <int KIND, int CAP, int TT>
 __device__ __forceinline__ void superblock(const uint8_t* b0, const uint8_t* b1, const Act<KIND, CAP, TT>& x, int g, int t, const uint32_t* grid,
-                                           float (&acc)[4]) {
-  using Col = Columns<KIND, TT>;
+                                           float (&acc)[CAP / 2]) {
+  constexpr int TF = Act<KIND, CAP, TT>::TF, NT = TT > 8 ? 2 : 1;
+  using Col = Columns<KIND, TF>;
   constexpr int NJ = Col::NJ, NC = Col::NC;
   const int fed = Col::fed_part(g), part0 = Col::part(t, 0), part1 = Col::part(t, 1);   // (parts within a fragment)
   // what the rows' scales come from
@@ -191,9 +200,9 @@ __device__ __forceinline__ void superblock(const uint8_t* b0, const uint8_t* b1,
     const float d = row ? d1 : d0;
     if constexpr (KIND == Q4K) {
       // (the parity of the slice says which nibble: odd ones are 16 times too large)
-      const bool upper = TT == 1 ? p >= 4 : TT == 2 ? f : TT == 4 ? f >> 1 : f >> 2;
-      const uint32_t at = TT == 1 ? p & 3 : TT == 2 ? p : TT == 4 ? (f & 1) * 2 + p : f & 3;
-      const bool odd = TT == 8 ? f & 1 : TT == 1 ? c : p & 1;
+      const bool upper = TF == 1 ? p >= 4 : TF == 2 ? f : TF == 4 ? f >> 1 : f >> 2;
+      const uint32_t at = TF == 1 ? p & 3 : TF == 2 ? p : TF == 4 ? (f & 1) * 2 + p : f & 3;
+      const bool odd = TF == 8 ? f & 1 : TF == 1 ? c : p & 1;
       const float e = odd ? 0.0625f * d : d;
       return fmaf(byte_on_2_23(sc[row], upper, at), e, -8388608.0f * e);
     } else if constexpr (KIND == IQ4XS) {
@@ -211,20 +220,23 @@ __device__ __forceinline__ void superblock(const uint8_t* b0, const uint8_t* b1,
   // raw words that several slices share
   uint2 q4[2];
   uint32_t l6[2][2][2], h6[2][2];
-  int half[4];
-  float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  int half[4 * NT];
+  float part[4 * NT] = {};
 #pragma unroll
   for (int f = 0; f < NC; ++f) {
-    constexpr int START = KIND == Q6K && TT == 8 ? 0 : MAGIC;
-    int c[4] = {START, START, START, START};
-    uint2 fed_words = make_uint2(0, 0);
-    if constexpr (KIND == Q6K) fed_words.x = x.quants16(f);
-    else fed_words = x.quants(f);
+    constexpr int START = KIND == Q6K && TF == 8 ? 0 : MAGIC;
+    int c[NT][4];
+    uint2 fed_words[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      c[n][0] = c[n][1] = c[n][2] = c[n][3] = START;
+      if constexpr (KIND == Q6K) fed_words[n] = make_uint2(x.quants16(f, n), 0);
+      else fed_words[n] = x.quants(f, n);
+    }
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const int s = f * NJ + j;        // part of the superblock
-      uint2 b = fed_words;
-      if (TT < 8 && fed != j) b = make_uint2(0, 0);
+      auto fed_now = [&](int n) { return TF < 8 && fed != j ? make_uint2(0, 0) : fed_words[n]; };
       uint32_t a[4];
       if constexpr (KIND == Q4K) {
         if ((s & 1) == 0) {
@@ -236,7 +248,8 @@ __device__ __forceinline__ void superblock(const uint8_t* b0, const uint8_t* b1,
         a[1] = q4[1].x & m;
         a[2] = q4[0].y & m;
         a[3] = q4[1].y & m;
-        mma_k32<true>(c, a, b);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_k32<true>(c[n], a, fed_now(n));
       } else if constexpr (KIND == IQ4XS) {
         const uint32_t t0 = reinterpret_cast<const uint32_t*>(c_iq4)[0], t1 = reinterpret_cast<const uint32_t*>(c_iq4)[1],
                        t2 = reinterpret_cast<const uint32_t*>(c_iq4)[2], t3 = reinterpret_cast<const uint32_t*>(c_iq4)[3];
@@ -248,7 +261,8 @@ __device__ __forceinline__ void superblock(const uint8_t* b0, const uint8_t* b1,
         };
         look_up(lds32(b0 + 8 + 16 * s + 4 * t), a[0], a[2]);
         look_up(lds32(b1 + 8 + 16 * s + 4 * t), a[1], a[3]);
-        mma_k32<false>(c, a, b);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_k32<false>(c[n], a, fed_now(n));
       } else if constexpr (KIND == IQ3S) {
         auto value = [&](uint32_t low, uint32_t high, uint32_t signs) {   // index low | high << 8, negated where a sign bit is set
           const uint32_t v = grid[(low | (high << 8)) * GRID_COPIES];
@@ -261,7 +275,8 @@ __device__ __forceinline__ void superblock(const uint8_t* b0, const uint8_t* b1,
         a[1] = value(q1 & 255u, e1 & 1u, g1);
         a[2] = value(q0 >> 8, (e0 >> 1) & 1u, g0 >> 4);
         a[3] = value(q1 >> 8, (e1 >> 1) & 1u, g1 >> 4);
-        mma_k32<false>(c, a, b);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_k32<false>(c[n], a, fed_now(n));
       } else {
         // part s: half s % 2 of slice s / 2. A value less 32 (six bits) is taken as q << 2 with the top bit flipped: four times it, as
         // a signed byte
@@ -283,71 +298,91 @@ __device__ __forceinline__ void superblock(const uint8_t* b0, const uint8_t* b1,
           const uint32_t hi = q == 3 ? h6[row][e] : h6[row][e] << (6 - 2 * q);
           return (lo & 0x3C3C3C3Cu) | ((hi & 0xC0C0C0C0u) ^ 0x80808080u);
         };
-        mma_k16(c, word(0), word(1), b.x);
+        const uint32_t a0 = word(0), a1 = word(1);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_k16(c[n], a0, a1, fed_now(n).x);
       }
     }
-    const float2 d = x.scales(f);
-    if constexpr (KIND == Q6K && TT == 8) {
+    if constexpr (KIND == Q6K && TF == 8) {
       // halves of a slice: sum_a * scale_a + sum_b * scale_b as integers, converted once, scaled by d at the end
       const int u0 = *reinterpret_cast<const int8_t*>(b0 + 192 + f), u1 = *reinterpret_cast<const int8_t*>(b1 + 192 + f);
-      const int n0 = u0 * c[0], n1 = u0 * c[1], n2 = u1 * c[2], n3 = u1 * c[3];
-      if (f & 1) {
-        part[0] = fmaf((float)(half[0] + n0), d.x, part[0]);
-        part[1] = fmaf((float)(half[1] + n1), d.y, part[1]);
-        part[2] = fmaf((float)(half[2] + n2), d.x, part[2]);
-        part[3] = fmaf((float)(half[3] + n3), d.y, part[3]);
-      } else {
-        half[0] = n0;
-        half[1] = n1;
-        half[2] = n2;
-        half[3] = n3;
-      }
-      if (f == NC - 1) {
-        acc[0] = fmaf(d0, part[0], acc[0]);
-        acc[1] = fmaf(d0, part[1], acc[1]);
-        acc[2] = fmaf(d1, part[2], acc[2]);
-        acc[3] = fmaf(d1, part[3], acc[3]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int n0 = u0 * c[n][0], n1 = u0 * c[n][1], n2 = u1 * c[n][2], n3 = u1 * c[n][3];
+        int* h = half + 4 * n;
+        float *p = part + 4 * n, *to = acc + 4 * n;
+        if (f & 1) {
+          const float2 d = x.scales(f, n);
+          p[0] = fmaf((float)(h[0] + n0), d.x, p[0]);
+          p[1] = fmaf((float)(h[1] + n1), d.y, p[1]);
+          p[2] = fmaf((float)(h[2] + n2), d.x, p[2]);
+          p[3] = fmaf((float)(h[3] + n3), d.y, p[3]);
+        } else {
+          h[0] = n0;
+          h[1] = n1;
+          h[2] = n2;
+          h[3] = n3;
+        }
+        if (f == NC - 1) {
+          to[0] = fmaf(d0, p[0], to[0]);
+          to[1] = fmaf(d0, p[1], to[1]);
+          to[2] = fmaf(d1, p[2], to[2]);
+          to[3] = fmaf(d1, p[3], to[3]);
+        }
       }
       continue;
     }
-    const float a00 = row_scale(0, f, 0), a10 = row_scale(1, f, 0), a01 = TT == 1 ? row_scale(0, f, 1) : a00, a11 = TT == 1 ? row_scale(1, f, 1) : a10;
-    acc[0] = fmaf(fmaf(__int_as_float(c[0]), a00, -MAGIC_F * a00), d.x, acc[0]);
-    acc[1] = fmaf(fmaf(__int_as_float(c[1]), a01, -MAGIC_F * a01), d.y, acc[1]);
-    acc[2] = fmaf(fmaf(__int_as_float(c[2]), a10, -MAGIC_F * a10), d.x, acc[2]);
-    acc[3] = fmaf(fmaf(__int_as_float(c[3]), a11, -MAGIC_F * a11), d.y, acc[3]);
-    if constexpr (KIND == Q4K && TT <= 2) {
+    const float a00 = row_scale(0, f, 0), a10 = row_scale(1, f, 0), a01 = TF == 1 ? row_scale(0, f, 1) : a00, a11 = TF == 1 ? row_scale(1, f, 1) : a10;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float2 d = x.scales(f, n);
+      float* to = acc + 4 * n;
+      to[0] = fmaf(fmaf(__int_as_float(c[n][0]), a00, -MAGIC_F * a00), d.x, to[0]);
+      to[1] = fmaf(fmaf(__int_as_float(c[n][1]), a01, -MAGIC_F * a01), d.y, to[1]);
+      to[2] = fmaf(fmaf(__int_as_float(c[n][2]), a10, -MAGIC_F * a10), d.x, to[2]);
+      to[3] = fmaf(fmaf(__int_as_float(c[n][3]), a11, -MAGIC_F * a11), d.y, to[3]);
+    }
+    if constexpr (KIND == Q4K && TF <= 2) {
       const float n0 = -h2f(h0.x >> 16), n1 = -h2f(h1.x >> 16);
       const float2 xs = x.quant_sums(f);
       auto low = [&](int row, int p) {
-        return (row ? n1 : n0) * (byte_on_2_23(mn[row], TT == 1 ? p >= 4 : f, TT == 1 ? p & 3 : p) - 8388608.0f);
+        return (row ? n1 : n0) * (byte_on_2_23(mn[row], TF == 1 ? p >= 4 : f, TF == 1 ? p & 3 : p) - 8388608.0f);
       };
-      const float m00 = low(0, part0), m10 = low(1, part0), m01 = TT == 1 ? low(0, part1) : m00, m11 = TT == 1 ? low(1, part1) : m10;
+      const float m00 = low(0, part0), m10 = low(1, part0), m01 = TF == 1 ? low(0, part1) : m00, m11 = TF == 1 ? low(1, part1) : m10;
       acc[0] = fmaf(m00, xs.x, acc[0]);
       acc[1] = fmaf(m01, xs.y, acc[1]);
       acc[2] = fmaf(m10, xs.x, acc[2]);
       acc[3] = fmaf(m11, xs.y, acc[3]);
     }
   }
-  if constexpr (KIND == Q4K && TT >= 4) {
+  if constexpr (KIND == Q4K && TF >= 4) {
     // rows g, g + 8 by slices t, t + 4; the sums' columns are the tokens (of 4 tokens, lanes t < 2 have them)
     auto low = [&](uint32_t w) { return __float_as_uint(__uint_as_float(prmt(w, 0x4B000000u, 0x7440u | t)) - 8388608.0f); };
     const uint32_t m0 = low(mn[0][0]), m1 = low(mn[1][0]), m2 = low(mn[0][1]), m3 = low(mn[1][1]);
-    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int p = 2; p >= 0; --p) mma_tf32(c, m0, m1, m2, m3, x.minima(p));
     const float n0 = -h2f(h0.x >> 16), n1 = -h2f(h1.x >> 16);
-    if (TT == 8 || t < 2) {
-      acc[0] = fmaf(n0, c[0], acc[0]);
-      acc[1] = fmaf(n0, c[1], acc[1]);
-      acc[2] = fmaf(n1, c[2], acc[2]);
-      acc[3] = fmaf(n1, c[3], acc[3]);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      // in three parts of at most 11 bits, the smallest first
+      const float2 xs = x.minima(n);
+      auto upper = [](float v) { return __uint_as_float(__float_as_uint(v) & 0xFFFFE000u); };
+      const float2 hi = make_float2(upper(xs.x), upper(xs.y)), r = make_float2(xs.x - hi.x, xs.y - hi.y), mid = make_float2(upper(r.x), upper(r.y));
+      float c[4] = {0.0f, 0.0f, 0.0f, 0.0f}, *to = acc + 4 * n;
+      mma_tf32(c, m0, m1, m2, m3, make_float2(r.x - mid.x, r.y - mid.y));
+      mma_tf32(c, m0, m1, m2, m3, mid);
+      mma_tf32(c, m0, m1, m2, m3, hi);
+      if (TF == 8 || t < 2) {
+        to[0] = fmaf(n0, c[0], to[0]);
+        to[1] = fmaf(n0, c[1], to[1]);
+        to[2] = fmaf(n1, c[2], to[2]);
+        to[3] = fmaf(n1, c[3], to[3]);
+      }
     }
   }
 }
 
 // A lane's sums over the parts that stood side by side: afterwards rows g, g + 8 by tokens 2 t, 2 t + 1.
-template <int TT>
-__device__ __forceinline__ void fold(float (&acc)[4]) {
+template <int TT, int N>
+__device__ __forceinline__ void fold(float (&acc)[N]) {
   if constexpr (TT == 1) {
     acc[0] += acc[1];
     acc[2] += acc[3];
@@ -363,7 +398,7 @@ __device__ __forceinline__ void fold(float (&acc)[4]) {
 // 8 quants of column `col` (words w0, w1; d: the scale of their 32, sum: the quants') into the staged activations. Whole warps call
 // it: four lanes share a slice of 32 values.
 template <int KIND, int CAP>
-__device__ __forceinline__ void stage_piece(uint32_t w0, uint32_t w1, float d, int piece, int col, int nsb, uint8_t* q_s, float* d_s, float* min_s) {
+__device__ __forceinline__ void stage_piece(uint32_t w0, uint32_t w1, float d, int piece, int col, uint8_t* q_s, float* d_s, float* sum_s) {
   const int s = piece >> 2, p = piece & 3;
   uint8_t* to = q_s + (s * CAP + col) * 32;
   if constexpr (KIND == Q6K) {           // lane t's words t and 4 + t side by side
@@ -380,25 +415,17 @@ __device__ __forceinline__ void stage_piece(uint32_t w0, uint32_t w1, float d, i
     int sum = dp4a((int)w0, 0x01010101, dp4a((int)w1, 0x01010101, 0));
     sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
     sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
-    if (p == 0) {                        // d * sum, and in three parts of at most 11 bits
-      const float xs = d * (float)sum, hi = __uint_as_float(__float_as_uint(xs) & 0xFFFFE000u), r = xs - hi;
-      const float mid = __uint_as_float(__float_as_uint(r) & 0xFFFFE000u);
-      min_s[s * CAP + col] = xs;
-      float* m = min_s + nsb * 8 * CAP + (s >> 3) * (CAP * 24) + (col * 4 + (s & 3)) * 2 + ((s >> 2) & 1);
-      m[0] = hi;
-      m[CAP * 8] = mid;
-      m[CAP * 16] = r - mid;
-    }
+    if (p == 0) sum_s[s * CAP + col] = d * (float)sum;
   }
   if (p == 0) d_s[s * CAP + col] = d;
 }
 
-// Stores a tile's sums: rows g, g + 8 by columns 2 t, 2 t + 1 of the group.
-template <bool DOWN>
-__device__ __forceinline__ void store_tile(const MoeArgs& a, const float (&acc)[4], int4 gr, int tile, const int* pair_s, const float* weight_s, int g, int t) {
+// Stores a tile's sums: rows g, g + 8 by columns 2 t, 2 t + 1 of the group (of its first 8 columns, then of the others).
+template <bool DOWN, int N>
+__device__ __forceinline__ void store_tile(const MoeArgs& a, const float (&acc)[N], int4 gr, int tile, const int* pair_s, const float* weight_s, int g, int t) {
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const int col = 2 * t + c;
+  for (int i = 0; i < N / 2; ++i) {
+    const int col = 8 * (i >> 1) + 2 * t + (i & 1), c = 4 * (i >> 1) + (i & 1);
     if (col < gr.z) {
       const int pair = pair_s[gr.w + col];
       if constexpr (DOWN) {
@@ -463,15 +490,16 @@ struct Place {
   }
 };
 
-// DOWN: rows of w2 on the activated products, else gate and up rows of w13 on X. STAGES: of a warp's ring; CAP: columns of activations.
-template <int KIND, bool DOWN, int STAGES, int CAP>
+// DOWN: rows of w2 on the activated products, else gate and up rows of w13 on X. SBS: superblocks of a stage; STAGES: of a warp's ring;
+// CAP: columns of activations, and the most pairs of a group.
+template <int KIND, bool DOWN, int SBS, int STAGES, int CAP>
 __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Window win;
   __shared__ int pair_s[CAP];
   __shared__ float weight_s[CAP];                    // (down product)
   __shared__ int token_s[CAP];                       // (gate / up product)
-  constexpr int PITCH = pitch(KIND), STAGE = 16 * PITCH, BS = bs(KIND), SBS = stage_sb(KIND);
+  constexpr int PITCH = pitch(KIND, SBS), STAGE = 16 * PITCH, BS = bs(KIND), A = CAP / 2;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int k = DOWN ? a.inter : a.hidden, rows = DOWN ? a.hidden : 2 * a.inter, tiles = rows >> 4, nsb = k >> 8, steps = (nsb + SBS - 1) / SBS;
   const int64_t rb = DOWN ? a.rb2 : a.rb13;
@@ -482,18 +510,18 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
   sp += (size_t)k * CAP;
   float* d_s = reinterpret_cast<float*>(sp);
   sp += (size_t)k / 32 * CAP * 4;
-  float* min_s = reinterpret_cast<float*>(sp);
-  if (KIND == Q4K) sp += (size_t)k / 256 * CAP * 128;
+  float* sum_s = reinterpret_cast<float*>(sp);       // d * sum of the quants (Q4_K)
+  if (KIND == Q4K) sp += (size_t)k / 32 * CAP * 4;
   uint32_t* grid_s = reinterpret_cast<uint32_t*>(sp);
   if (KIND == IQ3S) sp += 512 * 4 * GRID_COPIES;
-  float4* part_s = reinterpret_cast<float4*>(sp);    // [warps][lanes]: sums of the tile that begins before the warp's chunk
-  sp += WARPS * 512;
+  float4* part_s = reinterpret_cast<float4*>(sp);    // [warps][CAP / 8][lanes]: sums of the tile that begins before the warp's chunk
+  sp += WARPS * 64 * CAP;
   const uint8_t* ring = sp + (size_t)warp * STAGES * STAGE;
   // copies of a stage: copy i has pieces lane % 16 of rows 2 i and 2 i + 1, and where a row has more than 16 pieces one copy takes
   // pieces 16, 17 of all rows. Row r >= 8 of a gate / up tile is an up row.
   constexpr int PIECES = (SBS * BS + (KIND == Q4K ? 0 : KIND == IQ4XS ? 8 : 14) + 15) / 16;
   static_assert(PIECES <= 18 && 16 * PIECES <= PITCH, "");
-  const uint32_t to_rows = smem_addr(ring) + (lane >> 4) * PITCH + 16 * (lane & 15), to_rest = smem_addr(ring) + (lane >> 1) * PITCH + 256 + 16 * (lane & 1);
+  const uint32_t to_rows = smem_addr(ring) + row_place<KIND, SBS>(lane >> 4) * PITCH + 16 * (lane & 15), to_rest = smem_addr(ring) + (lane >> 1) * PITCH + 256 + 16 * (lane & 1);
   const uint8_t* const from_piece = weights + 16 * (lane & 15);
   const int64_t two_rows = 2 * rb, up_rows = DOWN ? 0 : (a.inter - 8) * rb, from_rows = (lane >> 4) * rb, from_rest = (lane >> 1) * rb + (lane >= 16 ? up_rows : 0);
 
@@ -513,8 +541,8 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
     for (int i = tid; i < 512 * GRID_COPIES; i += THREADS) grid_s[i] = g_iq3s[i / GRID_COPIES];
 
   for (; u0 < block_u1; u0 = win.end) {
-    // the window's groups, their columns and batches: a group's first column is even (its scales are read in pairs), and 8 columns from
-    // there on exist
+    // the window's groups, their columns and batches: a group's first column is even (its scales are read in pairs), and 8 or 16
+    // columns from there on exist
     __syncthreads();
     if (warp == 0) {
       const int first = u0 / tiles, n = min((block_u1 - 1) / tiles - first + 1, WINDOW);
@@ -525,7 +553,7 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
         int col = 0, b = 0;
         win.batch[0] = Batch{u0, end, 0, 0};
         for (int i = 0; i < n; ++i) {
-          if (col + 8 > CAP) {
+          if (col + (win.group[i].z > 8 ? 16 : 8) > CAP) {
             win.batch[b].u1 = (first + i) * tiles;
             win.batch[++b] = Batch{(first + i) * tiles, end, i, 0};
             col = 0;
@@ -555,9 +583,10 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
       if (in.live) {
         const bool half = SBS == 2 && 2 * in.step + 1 == nsb;      // (an odd row length: its last step is one superblock)
         const int bytes = half ? BS : SBS * BS;
-        // pieces 0 .. 15 of rows of two superblocks of 136 or 144 bytes, and 0 .. 13 of 210 bytes, are always needed
-        constexpr bool ALL = KIND == Q4K || KIND == IQ4XS || KIND == Q6K;
-        const bool mine = KIND != Q6K || (lane & 15) < 14;
+        // pieces that are always needed: of rows of 272 or 288 bytes 16 (and more, below), of 144 or 136 bytes (at 0 or 8) 9, of 210 bytes
+        // (at any even place) 14
+        constexpr bool ALL = KIND != IQ3S;
+        const bool mine = KIND == IQ3S || (lane & 15) < (KIND == Q6K ? 14 : SBS == 1 ? 9 : 16);
         auto copy = [&](uint32_t to, const uint8_t* from, int64_t row, int piece, bool sure) {
           if (sure || 16 * piece < (KIND == Q4K ? 0 : (int)(row & 15)) + bytes) copy16(to + slot * STAGE, from + (KIND == Q4K ? row : row & ~(int64_t)15));
         };
@@ -567,7 +596,7 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               if (i == 4) row += up_rows;
-              copy(to_rows + 2 * i * PITCH, from_piece, row, 0, true);
+              copy(to_rows + row_place<KIND, SBS>(2 * i) * PITCH, from_piece, row, 0, true);
               row += two_rows;
             }
           }
@@ -575,7 +604,7 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
 #pragma unroll 2
           for (int i = 0; i < 8; ++i) {
             if (i == 4) row += up_rows;
-            copy(to_rows + 2 * i * PITCH, from_piece, row, lane & 15, false);
+            copy(to_rows + row_place<KIND, SBS>(2 * i) * PITCH, from_piece, row, lane & 15, false);
             row += two_rows;
           }
         }
@@ -600,13 +629,14 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
         if (DOWN) asm volatile("griddepcontrol.wait;" ::: "memory");
         if (tid < CAP) pair_s[tid] = -1;
         __syncthreads();
-        if (tid < bt.n * 8) {
-          const int4 gr = win.group[bt.g0 + (tid >> 3)];
-          if ((tid & 7) < gr.z) {
-            const int pair = a.list[gr.y + (tid & 7)];
-            pair_s[gr.w + (tid & 7)] = pair;
-            if (DOWN) weight_s[gr.w + (tid & 7)] = a.weights[pair];
-            else token_s[gr.w + (tid & 7)] = pair / a.top_k;
+        if (tid < bt.n * CAP) {
+          const int4 gr = win.group[bt.g0 + tid / CAP];
+          const int i = tid % CAP;
+          if (i < gr.z) {
+            const int pair = a.list[gr.y + i];
+            pair_s[gr.w + i] = pair;
+            if (DOWN) weight_s[gr.w + i] = a.weights[pair];
+            else token_s[gr.w + i] = pair / a.top_k;
           }
         }
         __syncthreads();
@@ -650,19 +680,19 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
               w0 = moe_pack4(q[0], q[1], q[2], q[3]);
               w1 = moe_pack4(q[4], q[5], q[6], q[7]);
             }
-            stage_piece<KIND, CAP>(w0, w1, d[u], 32 * at_sb[u] + lane, at_col[u], nsb, q_s, d_s, min_s);
+            stage_piece<KIND, CAP>(w0, w1, d[u], 32 * at_sb[u] + lane, at_col[u], q_s, d_s, sum_s);
           }
         }
         __syncthreads();
       }
       int open_unit = -1;               // the tile that this warp has the beginning of, but not the end, and its sums so far
-      float open[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      float open[A] = {};
       while (at.live && at.batch == batch) {
         // a tile, or this warp's part of one
         const int group = at.group, tile = at.tile, unit = (win.first + group) * tiles + tile;
         const bool begins = at.step == 0;
         const int4 gr = win.group[group];
-        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        float acc[A] = {};
         uint32_t p0 = 0, p1 = 0;        // a row begins in its stage at what its offset is past a 16-byte boundary
         if (KIND != Q4K) {
           p0 = (uint32_t)row_offset(at, g);
@@ -671,14 +701,14 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
         bool ends = false;
         auto run = [&](auto tokens) {
           constexpr int TT = decltype(tokens)::value;
-          Act<KIND, CAP, TT> x(q_s, d_s, min_s, nsb, at.step * SBS, gr.w, g, t);
+          Act<KIND, CAP, TT> x(q_s, d_s, sum_s, at.step * SBS, gr.w, g, t);
           bool more = true;
           do {
             wait_all_but<STAGES - 2>();
             __syncwarp();               // every lane's pieces are there, and every lane is done with the stage before
             issue(slot == 0 ? STAGES - 1 : slot - 1);
-            const uint8_t* b0 = ring + slot * STAGE + g * PITCH + (KIND == Q4K ? 0 : p0 & 15);
-            const uint8_t* b1 = ring + slot * STAGE + (g + 8) * PITCH + (KIND == Q4K ? 0 : p1 & 15);
+            const uint8_t* b0 = ring + slot * STAGE + row_place<KIND, SBS>(g) * PITCH + (KIND == Q4K ? 0 : p0 & 15);
+            const uint8_t* b1 = ring + slot * STAGE + row_place<KIND, SBS>(g + 8) * PITCH + (KIND == Q4K ? 0 : p1 & 15);
             ends = at.step == steps - 1;
             const int n = SBS == 2 && (!ends || (nsb & 1) == 0) ? 2 : 1;
 #pragma unroll 1                        // (one copy of the code: a kernel starts with none of it in the instruction cache)
@@ -698,16 +728,18 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
         if (gr.z == 1) run(std::integral_constant<int, 1>());
         else if (gr.z == 2) run(std::integral_constant<int, 2>());
         else if (gr.z <= 4) run(std::integral_constant<int, 4>());
-        else run(std::integral_constant<int, 8>());
+        else if (CAP == 8 || gr.z <= 8) run(std::integral_constant<int, 8>());
+        else if constexpr (CAP > 8) run(std::integral_constant<int, 16>());
         if (begins && ends) {
           store_tile<DOWN>(a, acc, win.group[group], tile, pair_s, weight_s, g, t);
         } else {
           if (begins) {
             open_unit = unit;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) open[i] = acc[i];
+            for (int i = 0; i < A; ++i) open[i] = acc[i];
           } else {
-            part_s[warp * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+#pragma unroll
+            for (int i = 0; i < A / 4; ++i) part_s[(warp * (A / 4) + i) * 32 + lane] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
           }
         }
       }
@@ -717,8 +749,11 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
         for (int o = warp + 1, from = chunk_begin(bt, steps, o); from < tile_end; ++o) {
           const int to = chunk_begin(bt, steps, o + 1);
           if (to > from) {
-            const float4 q = part_s[o * 32 + lane];
-            open[0] += q.x; open[1] += q.y; open[2] += q.z; open[3] += q.w;
+#pragma unroll
+            for (int i = 0; i < A / 4; ++i) {
+              const float4 q = part_s[(o * (A / 4) + i) * 32 + lane];
+              open[4 * i] += q.x; open[4 * i + 1] += q.y; open[4 * i + 2] += q.z; open[4 * i + 3] += q.w;
+            }
           }
           from = to;
         }
@@ -733,53 +768,63 @@ static int kind_of(int type) {
   return type == GSQ_TYPE_Q4_K ? Q4K : type == GSQ_TYPE_Q6_K ? Q6K : type == GSQ_TYPE_IQ3_S ? IQ3S : type == GSQ_TYPE_IQ4_XS ? IQ4XS : -1;
 }
 
-// Columns of activations and stages of a warp's ring beside rows of k values. False: too long a row.
-static bool plan_of(int kind, int k, int max_smem, int* cap, int* stages, size_t* smem) {
-  const size_t room = (size_t)max_smem - 2304, stage = (size_t)WARPS * 16 * pitch(kind);   // (2304: the window, the columns and the driver's own)
-  const int plans[4][2] = {{16, 3}, {16, 2}, {8, 3}, {8, 2}};
-  for (const auto& p : plans) {
-    *cap = p[0];
-    *stages = p[1];
-    *smem = fixed_smem(kind, k, p[0]) + p[1] * stage;
-    if (*smem <= room) return true;
+// Columns of activations, superblocks of a stage and stages of a warp's ring beside rows of k values. Where experts have more than 4 pairs on
+// average (`many`), so that some have more than 8, 16 columns come before large stages: 16 tokens on one decoding of the weights (Q4_K,
+// 64 experts of 4096 x 2048: 314 us, in groups of 8 430); else the other way round (a token an expert: 171 us, 187 with stages
+// of one superblock). False: too long a row.
+struct Plan {
+  int cap, sbs, stages;
+  size_t smem;
+};
+static bool plan_of(int kind, int k, bool many, int max_smem, Plan* plan) {
+  const size_t room = (size_t)max_smem - 2304;   // (2304: the window, the columns and the driver's own)
+  static const int plans[2][4][3] = {{{16, 2, 2}, {8, 2, 2}, {8, 1, 3}, {8, 1, 2}}, {{16, 2, 2}, {16, 1, 3}, {8, 1, 3}, {8, 1, 2}}};
+  static const int plans_q6k[3][3] = {{16, 1, 3}, {16, 1, 2}, {8, 1, 2}};
+  for (int i = 0; i < (kind == Q6K ? 3 : 4); ++i) {
+    const int* p = kind == Q6K ? plans_q6k[i] : plans[many][i];
+    *plan = Plan{p[0], p[1], p[2], fixed_smem(kind, k, p[0]) + (size_t)p[2] * WARPS * 16 * pitch(kind, p[1])};
+    if (plan->smem <= room) return true;
   }
   return false;
 }
 
-template <int KIND, bool DOWN, int STAGES, int CAP>
-static int launch_kernel(const MoeArgs& a, size_t smem, int blocks, cudaStream_t st) {
-  GSQ_CUDA_TRY(cudaFuncSetAttribute(moe_mma_kernel<KIND, DOWN, STAGES, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  return moe_launch_behind(moe_mma_kernel<KIND, DOWN, STAGES, CAP>, blocks, THREADS, smem, st, a);
+template <int KIND, bool DOWN, int SBS, int STAGES, int CAP>
+static int launch_kernel(const MoeArgs& a, const Plan& p, cudaStream_t st) {
+  GSQ_CUDA_TRY(cudaFuncSetAttribute(moe_mma_kernel<KIND, DOWN, SBS, STAGES, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem));
+  return moe_launch_behind(moe_mma_kernel<KIND, DOWN, SBS, STAGES, CAP>, a.blocks, THREADS, p.smem, st, a);
 }
 
 template <int KIND, bool DOWN>
-static int launch(const MoeArgs& a, const DeviceInfo& di, cudaStream_t st) {
-  int cap, stages;
-  size_t smem;
-  if (!plan_of(KIND, DOWN ? a.inter : a.hidden, di.max_smem_optin, &cap, &stages, &smem)) return GSQ_ERR_UNSUPPORTED;
-  const int blocks = di.sm_count < MOE_BLOCKS ? di.sm_count : MOE_BLOCKS;
-  if (cap == 16) return stages == 3 ? launch_kernel<KIND, DOWN, 3, 16>(a, smem, blocks, st) : launch_kernel<KIND, DOWN, 2, 16>(a, smem, blocks, st);
-  return stages == 3 ? launch_kernel<KIND, DOWN, 3, 8>(a, smem, blocks, st) : launch_kernel<KIND, DOWN, 2, 8>(a, smem, blocks, st);
+static int launch(const MoeArgs& a, const Plan& p, cudaStream_t st) {
+  if constexpr (KIND == Q6K) {
+    if (p.cap == 8) return launch_kernel<KIND, DOWN, 1, 2, 8>(a, p, st);
+    return p.stages == 3 ? launch_kernel<KIND, DOWN, 1, 3, 16>(a, p, st) : launch_kernel<KIND, DOWN, 1, 2, 16>(a, p, st);
+  } else {
+    if (p.cap == 8 && p.sbs == 2) return launch_kernel<KIND, DOWN, 2, 2, 8>(a, p, st);
+    if (p.cap == 8) return p.stages == 3 ? launch_kernel<KIND, DOWN, 1, 3, 8>(a, p, st) : launch_kernel<KIND, DOWN, 1, 2, 8>(a, p, st);
+    return p.sbs == 2 ? launch_kernel<KIND, DOWN, 2, 2, 16>(a, p, st) : launch_kernel<KIND, DOWN, 1, 3, 16>(a, p, st);
+  }
 }
 
 }  // namespace moe
 
-// Whether the tensor-core kernel takes a product of this type and row length.
-bool moe_mma_serves(int type, int k) {
+// The most pairs of a group that the tensor-core kernel takes for this type and row length; 0: it does not take it.
+int moe_mma_serves(int type, int k, bool many) {
   const int kind = moe::kind_of(type);
   DeviceInfo di;
-  int cap, stages;
-  size_t smem;
-  return kind >= 0 && device_info(&di) == GSQ_OK && moe::plan_of(kind, k, di.max_smem_optin, &cap, &stages, &smem);
+  moe::Plan p;
+  return kind >= 0 && device_info(&di) == GSQ_OK && moe::plan_of(kind, k, many, di.max_smem_optin, &p) ? p.cap : 0;
 }
 
 int moe_mma_product(const MoeArgs& a, int type, bool down, cudaStream_t st) {
   DeviceInfo di;
-  const int rc = device_info(&di);
+  const int rc = device_info(&di), kind = moe::kind_of(type);
   if (rc != GSQ_OK) return rc;
+  moe::Plan p;
+  if (!moe::plan_of(kind, down ? a.inter : a.hidden, a.many, di.max_smem_optin, &p)) return GSQ_ERR_UNSUPPORTED;
 #define GSQ_MOE_KIND(K) \
-  case moe::K: return down ? moe::launch<moe::K, true>(a, di, st) : moe::launch<moe::K, false>(a, di, st);
-  switch (moe::kind_of(type)) {
+  case moe::K: return down ? moe::launch<moe::K, true>(a, p, st) : moe::launch<moe::K, false>(a, p, st);
+  switch (kind) {
     GSQ_MOE_KIND(Q4K)
     GSQ_MOE_KIND(Q6K)
     GSQ_MOE_KIND(IQ3S)
