@@ -100,17 +100,24 @@ def _act(name, g):
 
 def experts(x, raw13, raw2, t13, t2, weights, ids, act="silu", truncates=0.0):
     """(y, bound) float64 [tokens, hidden]: the layer's definition, and how far a sum in fp32 may be from it (before y is
-    rounded to its type). The bound follows the errors through: the gate and up products, the activation (four roundings and a
+    rounded to its type). The bound follows the errors through: the rounding of X to 8 bits, the gate and up products, the activation (four roundings and a
     function good to 2^-21), and the rounding of the activated product to 8 bits, where a value that is as near to a border as
     its own error may fall on either side. raw13 [experts][2 inter, bytes], raw2 [experts][hidden, bytes]."""
     m, hidden = x.shape
     y, bound = np.zeros((m, hidden)), np.zeros((m, hidden))
-    xq, xu, _ = q8(x)
+    xq, xu, xt = q8(x)
+    # 127 x, rounded to fp32, against half * amax, in one fused step: a quotient moves by its own 2^-24 before it is compared, and not at
+    # all where 127 x is an fp32 number (any 16-bit x)
+    x127 = 127.0 * np.asarray(x, dtype=np.float64)
+    xnear = (x127 != x127.astype(np.float32)) & (np.abs(np.abs(xt) - np.floor(np.abs(xt)) - 0.5) <= 1.01 * U32 * np.abs(xt))
+    xstep = xnear * np.repeat(xu, 32, -1)
     for e in sorted({int(i) for i in np.asarray(ids).ravel() if 0 <= i < len(raw13)}):
         toks, slots = np.nonzero(np.asarray(ids) == e)
         inter = raw13[e].shape[0] // 2
         gu = _product(raw13[e], t13, xq[toks], xu[toks])
         err = _sum_error(hidden) * _magnitudes(raw13[e], t13, xq[toks], xu[toks])
+        if xnear[toks].any():
+            err = err + xstep[toks] @ np.abs(values(raw13[e], t13)).T
         g, u, dg, du = gu[:, :inter], gu[:, inter:], err[:, :inter], err[:, inter:]
         a = _act(act, g)
         h = a * u
