@@ -762,7 +762,11 @@ static int launch_logprobs(const LogprobArgs& a, int64_t m, cudaStream_t st) {
   const int64_t rounds = (a.vocab / Vec<T>::N) / (LP_THREADS * LP_UNROLL);
   int cs = 1;
   while (cs < 16 && 2 * cs * m <= 2 * di.sm_count && cs <= rounds) cs *= 2;
-  if (cs > 8) GSQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  if (cs > 8) {
+    static OncePerDevice large;
+    const int set = large.set(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (set != GSQ_OK) return set;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(m * cs));
   cfg.blockDim = dim3(LP_THREADS);

@@ -774,7 +774,7 @@ static int kind_of(int type) {
 // of one superblock). False: too long a row.
 struct Plan {
   int cap, sbs, stages;
-  size_t smem;
+  size_t smem, room;         // of a block, and the most there is
 };
 static bool plan_of(int kind, int k, bool many, int max_smem, Plan* plan) {
   const size_t room = (size_t)max_smem - 2304;   // (2304: the window, the columns and the driver's own)
@@ -782,7 +782,7 @@ static bool plan_of(int kind, int k, bool many, int max_smem, Plan* plan) {
   static const int plans_q6k[3][3] = {{16, 1, 3}, {16, 1, 2}, {8, 1, 2}};
   for (int i = 0; i < (kind == Q6K ? 3 : 4); ++i) {
     const int* p = kind == Q6K ? plans_q6k[i] : plans[many][i];
-    *plan = Plan{p[0], p[1], p[2], fixed_smem(kind, k, p[0]) + (size_t)p[2] * WARPS * 16 * pitch(kind, p[1])};
+    *plan = Plan{p[0], p[1], p[2], fixed_smem(kind, k, p[0]) + (size_t)p[2] * WARPS * 16 * pitch(kind, p[1]), room};
     if (plan->smem <= room) return true;
   }
   return false;
@@ -790,7 +790,9 @@ static bool plan_of(int kind, int k, bool many, int max_smem, Plan* plan) {
 
 template <int KIND, bool DOWN, int SBS, int STAGES, int CAP>
 static int launch_kernel(const MoeArgs& a, const Plan& p, cudaStream_t st) {
-  GSQ_CUDA_TRY(cudaFuncSetAttribute(moe_mma_kernel<KIND, DOWN, SBS, STAGES, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem));
+  static OncePerDevice smem;
+  const int set = smem.set((const void*)moe_mma_kernel<KIND, DOWN, SBS, STAGES, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.room);
+  if (set != GSQ_OK) return set;
   return moe_launch_behind(moe_mma_kernel<KIND, DOWN, SBS, STAGES, CAP>, a.blocks, THREADS, p.smem, st, a);
 }
 

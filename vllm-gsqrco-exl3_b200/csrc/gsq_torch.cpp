@@ -10,6 +10,7 @@
 // (gsq_b200/quantization/linear.py `_lcpp_op`, restated in route() below and compared with it point by point in
 // tests/test_host_ops.py), buffers from torch's caching allocator on the current stream.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -556,9 +557,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& 
   TORCH_CHECK(token_ids.device() == logits.device(), op, ": all tensors must be on the logits' device");
   const c10::cuda::CUDAGuard dev(logits.device());
   const Tensor ids = token_ids.to(at::kLong).contiguous();
-  const auto f32 = logits.options().dtype(at::kFloat), i64 = logits.options().dtype(at::kLong);
-  Tensor lp = at::empty({m}, f32), rank = at::empty({m}, i64), entropy = at::empty({m}, f32), top = at::empty({m, top_n}, f32),
-         top_ids = at::empty({m, top_n}, i64);
+  const auto fresh = [&](at::IntArrayRef sizes, at::ScalarType type) { return at::detail::empty_cuda(sizes, type, logits.device(), std::nullopt); };
+  Tensor lp = fresh({m}, at::kFloat), rank = fresh({m}, at::kLong), entropy = fresh({m}, at::kFloat), top = fresh({m, top_n}, at::kFloat),
+         top_ids = fresh({m, top_n}, at::kLong);   // (past the dispatcher: five tensors a call)
   if (m)
     check(gsq_token_logprobs(logits.const_data_ptr(), dtype_code(logits.scalar_type()), m, vocab, row_stride(logits, vocab),
                              (const int64_t*)ids.const_data_ptr(), (int)top_n, (float*)lp.mutable_data_ptr(), (int64_t*)rank.mutable_data_ptr(),
