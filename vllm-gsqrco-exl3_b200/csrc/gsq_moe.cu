@@ -210,6 +210,7 @@ static int launch_quant(const void* x, int dtype, int vec, int64_t stride, int64
 constexpr int COMBINE_THREADS = 64;               // (a token's 2048 values on 8 SMs)
 __global__ void __launch_bounds__(COMBINE_THREADS) moe_combine_kernel(const MoeArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int per_row = a.hidden >> 2;
   const int64_t i = (int64_t)blockIdx.x * COMBINE_THREADS + threadIdx.x, t = i / per_row;
   if (t >= a.m) return;
@@ -256,6 +257,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) moe_plan_kernel(const MoeArgs a,
   __shared__ int place[GSQ_MOE_MAX_EXPERTS], cost_upto[GSQ_MOE_MAX_EXPERTS], group_upto[GSQ_MOE_MAX_EXPERTS];
   __shared__ int3 warp_sum[PLAN_WARPS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, pairs = a.m * a.top_k, experts = a.experts;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (blockIdx.x > 0) {                                          // the other blocks quantise X meanwhile
     const int64_t i = (int64_t)(blockIdx.x - 1) * PLAN_THREADS + tid;
@@ -440,12 +442,10 @@ constexpr int64_t PLAN_ROUTES = 64, PLAN_EXPERTS = 256;
 
 static int launch_plan(const MoeArgs& a, const RouteArgs* r, cudaStream_t st) {
   const unsigned grid = 1 + (unsigned)(((int64_t)a.m * (a.hidden >> 3) + PLAN_THREADS - 1) / PLAN_THREADS);
-  if (!r) moe_plan_kernel<0><<<grid, PLAN_THREADS, 0, st>>>(a, RouteArgs{});
-  else if (a.experts <= 64) moe_plan_kernel<2><<<grid, PLAN_THREADS, 0, st>>>(a, *r);
-  else if (a.experts <= 128) moe_plan_kernel<4><<<grid, PLAN_THREADS, 0, st>>>(a, *r);
-  else moe_plan_kernel<8><<<grid, PLAN_THREADS, 0, st>>>(a, *r);
-  GSQ_CUDA_TRY(cudaGetLastError());
-  return GSQ_OK;
+  if (!r) return moe_launch_behind(moe_plan_kernel<0>, grid, PLAN_THREADS, 0, st, a, RouteArgs{});
+  if (a.experts <= 64) return moe_launch_behind(moe_plan_kernel<2>, grid, PLAN_THREADS, 0, st, a, *r);
+  if (a.experts <= 128) return moe_launch_behind(moe_plan_kernel<4>, grid, PLAN_THREADS, 0, st, a, *r);
+  return moe_launch_behind(moe_plan_kernel<8>, grid, PLAN_THREADS, 0, st, a, *r);
 }
 
 // route: the choice to be made here, or NULL where ids and weights are there.
