@@ -240,11 +240,16 @@ __global__ void __launch_bounds__(COMBINE_THREADS) moe_combine_kernel(const MoeA
 // What a tile of the groups of n pairs costs, in 256ths of one of a single token (in 16ths, the blocks' shares of few experts were as coarse as a
 // share): as measured on groups of 1, 2, 4 and 8 (Q4_K 174, 190,
 // 193, 220 us for one layer; the other types differ less) and of 16 (1.4 times 8; the others 1.2).
-constexpr int COST_8 = 320, COST_16 = 416;
-__device__ __forceinline__ int moe_cost(int n, int group_max) {
-  const int r = n & (group_max - 1);
-  return (group_max == 8 ? (n >> 3) * COST_8 : (n >> 4) * COST_16) + (r == 0 ? 0 : r == 1 ? 256 : r == 2 ? 272 : r <= 4 ? 288 : r <= 8 ? COST_8 : COST_16);
-}
+// A block that goes on to another group stages its columns first and starts its pipelines anew: counted as `lead` tiles in front of the
+// group's own, one for each pair. (8 experts with 7 tokens on average, 148 blocks: the few that have the end of one group and the
+// beginning of the next were done at 47 us, the others at 39. The layer with no lead, a quarter, a half, one tile a pair: 72.2, 70.8, 67.2,
+// 62.5 us; 64 tokens of 64 experts: 275, 271, 270, 273.)
+struct GroupCost {
+  int group_max, tiles;                           // tiles of a group: the mean of the two products'
+  __device__ __forceinline__ int of_tiles(int n) const { return n == 1 ? 256 : n == 2 ? 272 : n <= 4 ? 288 : n <= 8 ? 320 : 416; }
+  __device__ __forceinline__ int lead(int n) const { return of_tiles(n) * n / tiles; }
+  __device__ __forceinline__ int of(int n) const { return of_tiles(n) + lead(n); }
+};
 
 // Pairs by expert: group, list, bounds. Block 0; PER_LANE > 0: it makes the choice first (few tokens). An expert's pairs stay in
 // their order, so that the same ones share a group every time (a group's size decides the order of its sums). Everything behind it
@@ -255,6 +260,7 @@ template <int PER_LANE>
 __global__ void __launch_bounds__(PLAN_THREADS) moe_plan_kernel(const MoeArgs a, const RouteArgs r) {
   __shared__ uint8_t of_warp[PLAN_WARPS][GSQ_MOE_MAX_EXPERTS];   // an expert's pairs among a warp's 32
   __shared__ int place[GSQ_MOE_MAX_EXPERTS], cost_upto[GSQ_MOE_MAX_EXPERTS], group_upto[GSQ_MOE_MAX_EXPERTS];
+  __shared__ uint8_t last_of[GSQ_MOE_MAX_EXPERTS];               // pairs of an expert's last group, where it is not a full one
   __shared__ int3 warp_sum[PLAN_WARPS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, pairs = a.m * a.top_k, experts = a.experts;
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -304,7 +310,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) moe_plan_kernel(const MoeArgs a,
     __syncthreads();
   }
   // sums over the experts before: pairs, groups, cost
-  const int most = a.group_max, g = (n + most - 1) >> (most == 8 ? 3 : 4), cost = moe_cost(n, most);
+  const int most = a.group_max, most_bits = most == 8 ? 3 : 4, g = (n + most - 1) >> most_bits;
+  const GroupCost group_cost{most, (a.inter >> 4) + (a.hidden >> 5)};
+  const int full = group_cost.of(most), last = n & (most - 1), cost = (n >> most_bits) * full + (last ? group_cost.of(last) : 0);
   int3 upto = make_int3(n, g, cost);
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -326,6 +334,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) moe_plan_kernel(const MoeArgs a,
   place[tid] = upto.x - n;
   cost_upto[tid] = upto.z;
   group_upto[tid] = upto.y;
+  last_of[tid] = (uint8_t)last;
   for (int i = 0; i < g; ++i) a.group[upto.y - g + i] = make_int4(tid, upto.x - n + most * i, min(most, n - most * i), 0);
   __syncthreads();
 
@@ -333,7 +342,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) moe_plan_kernel(const MoeArgs a,
   for (int b = tid; b <= a.blocks; b += PLAN_THREADS) {
     int2 at = make_int2(groups, 0);
     if (b < a.blocks && total > 0) {
-      const int target = (int)((uint32_t)total * b / a.blocks);   // (total: at most 32768 * 256 = 2^23, b up to 2^8)
+      const int target = (int)((uint32_t)total * b / a.blocks);   // (total: below 2^22, 5120 groups; b up to 2^8)
       int lo = 0, hi = experts - 1;
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
@@ -341,10 +350,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) moe_plan_kernel(const MoeArgs a,
         else lo = mid + 1;
       }
       // its groups: full ones, then the rest
-      const int full = most == 8 ? COST_8 : COST_16, first = lo ? group_upto[lo - 1] : 0, before = lo ? cost_upto[lo - 1] : 0, in = target - before;
+      const int first = lo ? group_upto[lo - 1] : 0, before = lo ? cost_upto[lo - 1] : 0, in = target - before;
       const int i = min(in / full, group_upto[lo] - first - 1), rest = in - i * full;
       const int whole = min(full, cost_upto[lo] - before - i * full);
-      at = make_int2(first + i, (rest << 16) / whole);
+      const int lead = whole == full ? group_cost.lead(most) : whole - group_cost.of_tiles(last_of[lo]);
+      at = make_int2(first + i, (max(rest - lead, 0) << 16) / (whole - lead));
     }
     a.bounds[b] = at;
   }
