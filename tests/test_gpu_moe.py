@@ -151,7 +151,8 @@ def test_strides_and_alignment():
         assert torch.equal(fused_moe.fused_moe_gguf(view, a, b, wd, idd, 12, 14), want)
     rows = xd[:1].expand(4, -1)                  # one token four times, row stride 0
     y = fused_moe.fused_moe_gguf(rows, a, b, wd[:1].expand(4, -1), idd[:1].expand(4, -1), 12, 14)
-    assert torch.equal(y, want[:1].expand(4, -1))
+    # (not `want`: other tokens beside it make other groups, and so another order of the sums)
+    assert torch.equal(y, fused_moe.fused_moe_gguf(rows.contiguous(), a, b, wd[:1].repeat(4, 1), idd[:1].repeat(4, 1), 12, 14))
     y = fused_moe.fused_moe_gguf(xd, a, b, wd.t().contiguous().t(), idd.t().contiguous().t(), 12, 14)   # the other order
     assert torch.equal(y, want)
     y = fused_moe.fused_moe_gguf(xd, a, b, wd.double(), idd.long(), 12, 14)

@@ -237,16 +237,15 @@ __global__ void __launch_bounds__(COMBINE_THREADS) moe_combine_kernel(const MoeA
   store_out_dyn(a.y, a.x_dtype, at + 3, s.w);
 }
 
-// What a tile of the groups of n pairs costs, in 256ths of one of a single token (in 16ths, the blocks' shares of few experts were as coarse as a
-// share): as measured on groups of 1, 2, 4 and 8 (Q4_K 174, 190,
-// 193, 220 us for one layer; the other types differ less) and of 16 (1.4 times 8; the others 1.2).
+// What a group costs: its tiles, at moe_mma_rates' rates.
 // A block that goes on to another group stages its columns first and starts its pipelines anew: counted as `lead` tiles in front of the
 // group's own, one for each pair. (8 experts with 7 tokens on average, 148 blocks: the few that have the end of one group and the
 // beginning of the next were done at 47 us, the others at 39. The layer with no lead, a quarter, a half, one tile a pair: 72.2, 70.8, 67.2,
 // 62.5 us; 64 tokens of 64 experts: 275, 271, 270, 273.)
 struct GroupCost {
-  int group_max, tiles;                           // tiles of a group: the mean of the two products'
-  __device__ __forceinline__ int of_tiles(int n) const { return n == 1 ? 256 : n == 2 ? 272 : n <= 4 ? 288 : n <= 8 ? 320 : 416; }
+  const int* rate;
+  int tiles;                                      // of a group: the mean of the two products'
+  __device__ __forceinline__ int of_tiles(int n) const { return rate[n <= 2 ? n - 1 : n <= 4 ? 2 : n <= 8 ? 3 : 4]; }
   __device__ __forceinline__ int lead(int n) const { return of_tiles(n) * n / tiles; }
   __device__ __forceinline__ int of(int n) const { return of_tiles(n) + lead(n); }
 };
@@ -311,7 +310,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) moe_plan_kernel(const MoeArgs a,
   }
   // sums over the experts before: pairs, groups, cost
   const int most = a.group_max, most_bits = most == 8 ? 3 : 4, g = (n + most - 1) >> most_bits;
-  const GroupCost group_cost{most, (a.inter >> 4) + (a.hidden >> 5)};
+  const GroupCost group_cost{a.rate, (a.inter >> 4) + (a.hidden >> 5)};
   const int full = group_cost.of(most), last = n & (most - 1), cost = (n >> most_bits) * full + (last ? group_cost.of(last) : 0);
   int3 upto = make_int3(n, g, cost);
 #pragma unroll
@@ -493,6 +492,7 @@ static int run_experts(const gsq_moe* w, const void* x, int x_dtype, int64_t m, 
   a.part = (float*)(ws + l.part);
   a.many = m * top_k > 4 * w->experts;
   const int up_mma = moe_mma_serves(w->w13_type, a.hidden, a.many), down_mma = moe_mma_serves(w->w2_type, a.inter, a.many);
+  moe_mma_rates(up_mma ? w->w13_type : w->w2_type, a.rate);
   a.group_max = up_mma == 8 || down_mma == 8 ? 8 : 16;
   for (int64_t t0 = 0; t0 < m; t0 += PASS_TOKENS) {
     a.m = (int)(m - t0 < PASS_TOKENS ? m - t0 : PASS_TOKENS);

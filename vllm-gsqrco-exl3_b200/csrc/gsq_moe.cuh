@@ -30,6 +30,7 @@ struct MoeArgs {
   // pairs by expert, at most group_max (8 or 16) to a group
   int group_max;
   bool many;                   // pairs: more than 4 an expert on average
+  int rate[5];                 // cost of a tile of a group of 1, 2, up to 4, 8, 16 pairs
   int2* bounds;                // [blocks + 1]: where a block's share of (group, tile) begins: a group, and 65536ths of its tiles
   int blocks;                  // of the products
   int4* group;                 // expert, first place in the list, pairs
@@ -100,5 +101,6 @@ int moe_dot_down(const MoeArgs& a, int type, cudaStream_t st);
 // gsq_moe_mma.cu: the same by groups, from xq / xd to h, from h to part
 int moe_mma_serves(int type, int k, bool many);
 int moe_mma_product(const MoeArgs& a, int type, bool down, cudaStream_t st);
+void moe_mma_rates(int type, int (&rate)[5]);   // MoeArgs::rate
 
 }  // namespace gsq

@@ -1,29 +1,34 @@
 // The experts' products on the tensor cores, for the four main types (Q4_K, Q6_K, IQ3_S, IQ4_XS in GGUF order) (sm_100a).
 //
-// The pairs of a token and one of its experts are gathered by expert, at most 8 to a group (gsq_moe.cu), so that an expert's
-// weights are read and decoded once for 8 tokens. A tile is 16 weight rows: 8 gate and the 8 up rows of the same channels, which
+// The pairs of a token and one of its experts are gathered by expert, at most 8 or 16 to a group (gsq_moe.cu), so that an expert's
+// weights are read and decoded once for them. A tile is 16 weight rows: 8 gate and the 8 up rows of the same channels, which
 // leaves a channel's gate and up sums in one lane, or 16 rows of the down weights. The list of (group, tile) is cut into one
 // contiguous range a block of equal estimated cost, one block an SM; a block takes as many groups of its range at a time as its columns of
 // activations hold (a batch, mostly all of them), and cuts the batch's superblocks into 16 equal contiguous chunks, one a warp.
 //
-//   * Weights: each warp has a ring of asynchronous copies of its own (a stage is 16 rows x 2 superblocks, 1 for Q6_K; 16 lanes copy
-//     consecutive 16-byte pieces of a row), filled ahead over tiles and batches, so the stream does not stop. Rows of 210- and 110-byte blocks start at any even address: copies begin at
-//     the 16-byte boundary before, and the rows are read at their offset. (One bulk copy a row was a loop over the 16 lanes that
-//     issue them: 95 of 427 instructions a superblock.)
+//   * Weights: each warp has a ring of asynchronous copies of its own (a stage is 16 rows x 2 superblocks, or 1; 16 lanes copy
+//     consecutive 16-byte pieces of a row), filled ahead over tiles and batches, so the stream does not stop. Rows of 210- and 110-byte
+//     blocks start at any even address: copies begin at the 16-byte boundary before, and the rows are read at their offset. (One bulk
+//     copy a row was a loop over the 16 lanes that issue them: 95 of 427 instructions a superblock.)
 //   * Activations: the block takes its batch's rows (X in 8 bits, or the activated products, which it quantises) into shared memory in
-//     the order of the tensor-core instruction's B fragment. An instruction takes the 8 columns from its group's first on; what it finds past the
-//     group's own only reaches sums that are not stored.
+//     the order of the tensor-core instruction's B fragment. An instruction takes the 8 columns from its group's first on; what it finds
+//     past the group's own only reaches sums that are not stored. A group of more than 8 takes two instructions on one decoding.
 //   * Product: mma.sync m16n8k32 on bytes (m16n8k16 for Q6_K, whose sub-scales cover 16 values); a lane decodes exactly its share of
-//     the A fragment. Every sub-scale's sum has to be scaled on its own, and that, not the instruction, is the cost: with a column for
+//     the A fragment. tcgen05 has no 8-bit integer form, and every 32 values' sums are scaled on their own before they are added, which
+//     would read an accumulator out of TMEM once per slice. That scaling, not the instruction, is the cost: with a column for
 //     each of 8 tokens it is 14 instructions a slice and lane. A group of 1, 2 or 4 tokens therefore gives the free columns to other
 //     slices: the instruction of slice j has the activations in the columns of slice j and zeros in the others, and the sums of 8, 4
-//     or 2 slices come out side by side in one C fragment, scaled at once. (Q4_K, instructions a superblock of 16 rows: 357 with one
-//     form for all, of which DRAM's rate leaves room for 250.)
+//     or 2 slices come out side by side in one C fragment, scaled at once.
 //   * Sums leave the instruction on the bit pattern of 1.5 * 2^23, so fma(sum, dA, -1.5 * 2^23 dA) is the exact integer times
 //     d * sub-scale without a conversion; the second fma scales by the activations. Q4_K's high nibbles are multiplied where they
-//     are, as unsigned bytes 16 times their value. Its minima, for 4 and 8 tokens, are a product of their own, min [16 rows x 8
+//     are, as unsigned bytes 16 times their value. Its minima, for 4 tokens and more, are a product of their own, min [16 rows x 8
 //     slices] times d_x * sum of the quants [8 slices x 8 columns], in three tf32 parts that hold all 24 bits.
 //   * A tile that several warps have parts of is added up by the warp that has its beginning, in the order of the warps.
+//
+// Measured, 64 experts of 4096 x 2048 with 1, 2, 4, 8, 16 tokens each, the whole layer (least time at the measured 6.54 TB/s in front): Q4_K 138:
+// 171, 174, 186, 220, 308 us; IQ4_XS 131: 266, 269, 296, 333, 405; Q6_K 202: 273, 337, 337, 316, 403; IQ3_S 106: 333, 348, 373, 396, 479. Q4_K
+// with one token an expert runs at DRAM's rate (85 % with the 25 us that a call takes besides); the others are bound by the
+// instructions that decode them (look-ups of 8 nibbles, 6-bit values put together, a codebook).
 #include <type_traits>
 
 #include "gsq_moe.cuh"
@@ -727,7 +732,7 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
         };
         if (gr.z == 1) run(std::integral_constant<int, 1>());
         else if (gr.z == 2) run(std::integral_constant<int, 2>());
-        else if (gr.z <= 4) run(std::integral_constant<int, 4>());
+        else if (KIND != Q6K && gr.z <= 4) run(std::integral_constant<int, 4>());   // (Q6_K, 4 tokens an expert: 347 us so, 337 in the form for 8)
         else if (CAP == 8 || gr.z <= 8) run(std::integral_constant<int, 8>());
         else if constexpr (CAP > 8) run(std::integral_constant<int, 16>());
         if (begins && ends) {
@@ -816,6 +821,15 @@ int moe_mma_serves(int type, int k, bool many) {
   DeviceInfo di;
   moe::Plan p;
   return kind >= 0 && device_info(&di) == GSQ_OK && moe::plan_of(kind, k, many, di.max_smem_optin, &p) ? p.cap : 0;
+}
+
+// What a tile costs, in 256ths of one of a single token, as seen on the blocks of layers with groups of different sizes. In 16ths, the shares of few
+// experts' blocks were as coarse as a share (27 tokens of 8 experts: 88 us, 74 in 256ths). Q6_K's form for two tokens is dear: with the
+// others' rates the blocks of such groups were done at 33 us, those of single tokens at 28 (8 tokens, half of 64 experts: 56 us, 53 with its
+// own).
+void moe_mma_rates(int type, int (&rate)[5]) {
+  static const int rates[2][5] = {{256, 272, 288, 320, 416}, {256, 320, 305, 305, 380}};
+  for (int i = 0; i < 5; ++i) rate[i] = rates[type == GSQ_TYPE_Q6_K][i];
 }
 
 int moe_mma_product(const MoeArgs& a, int type, bool down, cudaStream_t st) {
