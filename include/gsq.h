@@ -365,7 +365,7 @@ int gsq_peer_reduce_error_flag(int* flag);
  *   gsq_moe          the experts: w13 uint8 [experts, 2 * inter, bytes of `hidden` values], gate rows before up rows; w2 uint8
  *                    [experts, hidden, bytes of `inter` values]; GGUF order (not repacked), any of the ten types each, 16-byte
  *                    aligned; hidden and inter multiples of 256
- *   x, y             [m, hidden] in x_dtype, rows x_row_stride / y_row_stride elements apart; y apart from x
+ *   x, y             [m, hidden] in x_dtype (all pointers: aligned to their elements), rows x_row_stride / y_row_stride elements apart; y apart from x
  *   topk_weights, topk_ids   [m, top_k] contiguous; ids int32, or int64 with ids_64 != 0. An id outside [0, experts) is a choice
  *                    that is not here (another rank's): it adds nothing. A token without choices gets zeros. The same expert
  *                    twice counts twice.
@@ -411,7 +411,7 @@ int gsq_moe_layer(const gsq_moe* w, const void* x, int x_dtype, int64_t m, int64
 /*
  * What a server answers with behind the head: per row of logits [m, vocab] (dtype, rows row_stride elements apart) the log
  * probability of one given token, its rank, the row's entropy and the top_n (0..32) most probable tokens with their log
- * probabilities. Not in the reference (vLLM's sampler runs log_softmax, gather, a comparison and topk). Natural logarithms,
+ * probabilities. Pointers aligned to their elements. Not in the reference (vLLM's sampler runs log_softmax, gather, a comparison and topk). Natural logarithms,
  * statistics in fp32. Order of tokens: larger logit first, lower index first among equals, NaN last.
  *   token_ids      [m] int64. Negative: no token (log probability 0, rank 0). >= vocab: NaN, rank 0.
  *   logprobs [m], ranks [m] (1 = first in that order), entropy [m]

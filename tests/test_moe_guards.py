@@ -165,3 +165,21 @@ def test_c_entry_points_refuse_before_the_gpu():
 def test_empty_calls_on_the_host():
     with pytest.raises(RuntimeError, match="must be CUDA"):
         logprobs.token_logprobs(torch.zeros(0, 10), torch.zeros(0, dtype=torch.int64), 3)
+
+
+def test_c_entry_points_refuse_pointers_between_elements():
+    lib, at = _cabi.lib, C.c_void_p
+    g, size = _cabi.Moe(16, 16, 12, 14, 4, 512, 256, 0), lib.gsq_moe_workspace_bytes(3, 512, 256, 2)
+
+    def experts(x=256, y=256, weights=256, ids=256, ids_64=0, dtype=0):
+        return lib.gsq_moe_experts(C.byref(g), at(x), dtype, 3, 512, at(weights), at(ids), ids_64, 2, at(y), 512, at(256), size, None)
+
+    for kw in ({"x": 258}, {"x": 257, "dtype": 2}, {"y": 258}, {"y": 257, "dtype": 1}, {"weights": 258}, {"ids": 258}, {"ids": 260, "ids_64": 1}):
+        assert experts(**kw) == _cabi.ERR_UNSUPPORTED, kw
+    for logits, dtype, bias, weights, ids in ((258, 0, None, 256, 256), (257, 2, None, 256, 256), (256, 0, 258, 256, 256), (256, 0, None, 258, 256), (256, 0, None, 256, 258)):
+        r = _cabi.MoeRouter(logits, dtype, 8, 0, 1, bias, 1.0)
+        assert lib.gsq_moe_route(C.byref(r), 3, 8, 2, at(weights), at(ids), None) == _cabi.ERR_UNSUPPORTED
+    good = [256] * 7
+    for i, v in ((0, 257), (1, 260), (2, 258), (3, 260), (4, 258), (5, 258), (6, 260)):
+        p = [at(v if i == j else q) for j, q in enumerate(good)]
+        assert lib.gsq_token_logprobs(p[0], 2, 2, 100, 100, p[1], 3, p[2], p[3], p[4], p[5], p[6], None) == _cabi.ERR_UNSUPPORTED

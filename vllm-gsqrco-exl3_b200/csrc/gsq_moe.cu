@@ -223,7 +223,8 @@ __global__ void __launch_bounds__(COMBINE_THREADS) moe_combine_kernel(const MoeA
 #pragma unroll
     for (int u = 0; u < U; ++u) here[u] = r0 + u < a.top_k && moe_expert(a, (int)(t * a.top_k) + r0 + u) >= 0;
 #pragma unroll
-    for (int u = 0; u < U; ++u) p[u] = here[u] ? __ldcg(reinterpret_cast<const float4*>(a.part + (t * a.top_k + r0 + u) * a.hidden + c)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int u = 0; u < U; ++u)
+      p[u] = here[u] ? __ldcg(reinterpret_cast<const float4*>(a.part + (t * a.top_k + r0 + u) * a.hidden + c)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (here[u]) {
@@ -417,11 +418,15 @@ struct MoeLayout {
   }
 };
 
+static bool at_multiple(const void* p, size_t bytes) { return (uintptr_t)p % bytes == 0; }
+static size_t element_bytes(int dtype) { return dtype == GSQ_F32 ? 4 : 2; }
+
 static int check_router(const gsq_moe_router* r, int64_t m, int64_t experts, int top_k) {
   if (!r || !r->logits || m < 0 || experts <= 0 || top_k <= 0 || top_k > experts || r->row_stride < 0) return GSQ_ERR_UNSUPPORTED;
   if (experts > GSQ_MOE_MAX_EXPERTS || top_k > GSQ_MOE_MAX_TOP_K || m > INT32_MAX) return GSQ_ERR_TOO_LARGE;
   if (r->dtype != GSQ_F32 && r->dtype != GSQ_F16 && r->dtype != GSQ_BF16) return GSQ_ERR_UNSUPPORTED;
   if (r->scoring != GSQ_MOE_SOFTMAX && r->scoring != GSQ_MOE_SIGMOID) return GSQ_ERR_UNSUPPORTED;
+  if (!at_multiple(r->logits, element_bytes(r->dtype)) || !at_multiple(r->bias, 4)) return GSQ_ERR_UNSUPPORTED;
   return GSQ_OK;
 }
 
@@ -437,11 +442,12 @@ static int check_moe(const gsq_moe* w, const void* x, int x_dtype, int64_t m, in
   if (w->activation != GSQ_ACT_SILU && w->activation != GSQ_ACT_GELU) return GSQ_ERR_UNSUPPORTED;
   if (x_dtype != GSQ_F32 && x_dtype != GSQ_F16 && x_dtype != GSQ_BF16) return GSQ_ERR_UNSUPPORTED;
   if (m == 0) return GSQ_OK;
-  if (!w->w13 || !w->w2 || !x || !y || (uintptr_t)w->w13 % 16 || (uintptr_t)w->w2 % 16) return GSQ_ERR_UNSUPPORTED;
+  if (!w->w13 || !w->w2 || !x || !y || !at_multiple(w->w13, 16) || !at_multiple(w->w2, 16)) return GSQ_ERR_UNSUPPORTED;
+  if (!at_multiple(x, element_bytes(x_dtype)) || !at_multiple(y, element_bytes(x_dtype))) return GSQ_ERR_UNSUPPORTED;
   if (x_row_stride < 0 || (m > 1 && y_row_stride < w->hidden)) return GSQ_ERR_UNSUPPORTED;
   if (w->hidden > (1 << 17) || w->inter > (1 << 17) || w->experts > GSQ_MOE_MAX_EXPERTS || top_k > GSQ_MOE_MAX_TOP_K || m > GSQ_MOE_MAX_TOKENS)
     return GSQ_ERR_TOO_LARGE;
-  if (!ws || ws_bytes < gsq_moe_workspace_bytes(m, w->hidden, w->inter, top_k) || (uintptr_t)ws % 256) return GSQ_ERR_SCRATCH;
+  if (!ws || ws_bytes < gsq_moe_workspace_bytes(m, w->hidden, w->inter, top_k) || !at_multiple(ws, 256)) return GSQ_ERR_SCRATCH;
   return GSQ_OK;
 }
 
@@ -473,7 +479,7 @@ static int run_experts(const gsq_moe* w, const void* x, int x_dtype, int64_t m, 
   a.top_k = top_k;
   a.x_dtype = x_dtype;
   a.x_stride = x_row_stride;
-  const int64_t es = x_dtype == GSQ_F32 ? 4 : 2, id_bytes = ids64 ? 8 : 4;
+  const int64_t es = (int64_t)element_bytes(x_dtype), id_bytes = ids64 ? 8 : 4;
   a.x_vec = (uintptr_t)x % 16 == 0 && (m == 1 || x_row_stride * es % 16 == 0);
   a.ids64 = ids64;
   a.y_stride = y_row_stride;
@@ -520,7 +526,8 @@ static int run_experts(const gsq_moe* w, const void* x, int x_dtype, int64_t m, 
       if (rc == GSQ_OK) rc = moe_dot_down(a, w->w2_type, st);
     }
     if (rc != GSQ_OK) return rc;
-    rc = moe_launch_behind(moe_combine_kernel, (unsigned)(((int64_t)a.m * (a.hidden >> 2) + COMBINE_THREADS - 1) / COMBINE_THREADS), COMBINE_THREADS, 0, st, a);
+    const int64_t sums = (int64_t)a.m * (a.hidden >> 2);
+    rc = moe_launch_behind(moe_combine_kernel, (unsigned)((sums + COMBINE_THREADS - 1) / COMBINE_THREADS), COMBINE_THREADS, 0, st, a);
     if (rc != GSQ_OK) return rc;
   }
   return GSQ_OK;
@@ -538,7 +545,7 @@ extern "C" int gsq_moe_route(const gsq_moe_router* r, int64_t m, int64_t experts
   if (m == 0) return GSQ_OK;
   const int rc = gsq::check_router(r, m, experts, top_k);
   if (rc != GSQ_OK) return rc;
-  if (!topk_weights || !topk_ids) return GSQ_ERR_UNSUPPORTED;
+  if (!topk_weights || !topk_ids || !gsq::at_multiple(topk_weights, 4) || !gsq::at_multiple(topk_ids, 4)) return GSQ_ERR_UNSUPPORTED;
   return gsq::launch_route(gsq::route_args(r, m, experts, top_k, topk_weights, topk_ids), (cudaStream_t)stream);
 }
 
@@ -547,7 +554,7 @@ extern "C" int gsq_moe_experts(const gsq_moe* w, const void* x, int x_dtype, int
                                size_t workspace_bytes, void* stream) {
   const int rc = gsq::check_moe(w, x, x_dtype, m, x_row_stride, top_k, y, y_row_stride, workspace, workspace_bytes);
   if (rc != GSQ_OK || m == 0) return rc;
-  if (!topk_weights || !topk_ids) return GSQ_ERR_UNSUPPORTED;
+  if (!topk_weights || !topk_ids || !gsq::at_multiple(topk_weights, 4) || !gsq::at_multiple(topk_ids, ids_64 ? 8 : 4)) return GSQ_ERR_UNSUPPORTED;
   return gsq::run_experts(w, x, x_dtype, m, x_row_stride, topk_weights, topk_ids, ids_64, top_k, y, y_row_stride, (uint8_t*)workspace,
                           nullptr, (cudaStream_t)stream);
 }

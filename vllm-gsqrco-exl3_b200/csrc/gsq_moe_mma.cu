@@ -427,7 +427,8 @@ __device__ __forceinline__ void stage_piece(uint32_t w0, uint32_t w1, float d, i
 
 // Stores a tile's sums: rows g, g + 8 by columns 2 t, 2 t + 1 of the group (of its first 8 columns, then of the others).
 template <bool DOWN, int N>
-__device__ __forceinline__ void store_tile(const MoeArgs& a, const float (&acc)[N], int4 gr, int tile, const int* pair_s, const float* weight_s, int g, int t) {
+__device__ __forceinline__ void store_tile(const MoeArgs& a, const float (&acc)[N], int4 gr, int tile, const int* pair_s, const float* weight_s,
+                                           int g, int t) {
 #pragma unroll
   for (int i = 0; i < N / 2; ++i) {
     const int col = 8 * (i >> 1) + 2 * t + (i & 1), c = 4 * (i >> 1) + (i & 1);
@@ -526,9 +527,11 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
   // pieces 16, 17 of all rows. Row r >= 8 of a gate / up tile is an up row.
   constexpr int PIECES = (SBS * BS + (KIND == Q4K ? 0 : KIND == IQ4XS ? 8 : 14) + 15) / 16;
   static_assert(PIECES <= 18 && 16 * PIECES <= PITCH, "");
-  const uint32_t to_rows = smem_addr(ring) + row_place<KIND, SBS>(lane >> 4) * PITCH + 16 * (lane & 15), to_rest = smem_addr(ring) + (lane >> 1) * PITCH + 256 + 16 * (lane & 1);
+  const uint32_t to_rows = smem_addr(ring) + row_place<KIND, SBS>(lane >> 4) * PITCH + 16 * (lane & 15);
+  const uint32_t to_rest = smem_addr(ring) + (lane >> 1) * PITCH + 256 + 16 * (lane & 1);
   const uint8_t* const from_piece = weights + 16 * (lane & 15);
-  const int64_t two_rows = 2 * rb, up_rows = DOWN ? 0 : (a.inter - 8) * rb, from_rows = (lane >> 4) * rb, from_rest = (lane >> 1) * rb + (lane >= 16 ? up_rows : 0);
+  const int64_t two_rows = 2 * rb, up_rows = DOWN ? 0 : (a.inter - 8) * rb;
+  const int64_t from_rows = (lane >> 4) * rb, from_rest = (lane >> 1) * rb + (lane >= 16 ? up_rows : 0);
 
   // Launched while the kernel before runs (launch_kernel). The gate / up product waits for the plan; the down product has the plan from
   // before that product, and its first weights come in while that finishes.
@@ -744,7 +747,8 @@ __global__ void __launch_bounds__(THREADS, 1) moe_mma_kernel(const MoeArgs a) {
             for (int i = 0; i < A; ++i) open[i] = acc[i];
           } else {
 #pragma unroll
-            for (int i = 0; i < A / 4; ++i) part_s[(warp * (A / 4) + i) * 32 + lane] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+            for (int i = 0; i < A / 4; ++i)
+              part_s[(warp * (A / 4) + i) * 32 + lane] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
           }
         }
       }
