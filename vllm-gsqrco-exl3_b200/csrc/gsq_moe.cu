@@ -352,9 +352,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) moe_plan_kernel(const MoeArgs a,
       // its groups: full ones, then the rest
       const int first = lo ? group_upto[lo - 1] : 0, before = lo ? cost_upto[lo - 1] : 0, in = target - before;
       const int i = min(in / full, group_upto[lo] - first - 1), rest = in - i * full;
-      const int whole = min(full, cost_upto[lo] - before - i * full);
-      const int lead = whole == full ? group_cost.lead(most) : whole - group_cost.of_tiles(last_of[lo]);
-      at = make_int2(first + i, (max(rest - lead, 0) << 16) / (whole - lead));
+      const int size = first + i + 1 < group_upto[lo] || !last_of[lo] ? most : last_of[lo];
+      // rest < group_cost.of(size): below 65536, so that the boundary lies in the group
+      at = make_int2(first + i, (max(rest - group_cost.lead(size), 0) << 16) / group_cost.of_tiles(size));
     }
     a.bounds[b] = at;
   }
