@@ -181,3 +181,74 @@ def test_experts_of_all_ranks_add_up():
     ref, bound = moe.experts(x.float().numpy(), r13, r2, 12, 14, w.cpu().numpy(), ids.cpu().numpy())
     tol = bound + HALF_STEP[torch.bfloat16] * 1.01 * sum(np.abs(p) for p in parts) + 1e-7
     assert (np.abs(sum(parts) - ref) <= tol).all()
+
+
+def _two_ops():
+    """Inputs and calls of the layer and the log probabilities on the same buffers."""
+    from gsq_b200 import logprobs
+
+    x, r13, r2, logits, _, _ = _inputs(9, 12, 3, 1024, 512, "Q4_K", "Q6_K", torch.bfloat16, 98)
+    xd, a, b, ld = _cuda(x, r13, r2, logits)
+    vocab = torch.randn(9, 30000, device=DEV)
+    ids = torch.arange(9, device=DEV) * 3000
+
+    def call():
+        y = fused_moe.moe_layer_gguf(xd, ld, a, b, 12, 14, 3)
+        return (y, *logprobs.token_logprobs(vocab, ids, 5), *logprobs.token_logprobs(vocab[:, :1000], ids % 1000, 5))
+
+    return (xd, ld, vocab), call
+
+
+def test_inputs_written_by_the_kernel_before():
+    """The kernels start while the one before still runs: what that one writes, in place and into memory that a call before
+    has just given back, is what they read."""
+    buffers, call = _two_ops()
+    g = torch.Generator(device=DEV).manual_seed(5)
+    rounds = [[torch.randn(t.shape, device=DEV, generator=g).to(t.dtype) for t in buffers] for _ in range(12)]
+    want = []
+    for r in rounds:
+        for t, v in zip(buffers, r):
+            t.copy_(v)
+        torch.cuda.synchronize()
+        want.append(call())
+        torch.cuda.synchronize()
+    got = []
+    for r in rounds:
+        for t, v in zip(buffers, r):
+            t.copy_(v)
+        call()                                    # (its results' memory is free again for the next)
+        got.append(call())
+    assert all(torch.equal(p, q) for w, h in zip(want, got) for p, q in zip(w, h))
+
+
+def test_captured_behind_copies_and_other_streams():
+    """In a graph behind a fill, a copy and a join of two streams, and in front of a copy and of another stream's work."""
+    buffers, call = _two_ops()
+    new = [torch.randn(t.shape, device=DEV).to(t.dtype) for t in buffers]
+    for t, v in zip(buffers, new):
+        t.copy_(v)
+    want = call()
+    for t in buffers:
+        t.zero_()
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        buffers[0].zero_()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            buffers[2].copy_(new[2])
+        buffers[0].copy_(new[0])
+        buffers[1].copy_(new[1])
+        main.wait_stream(side)
+        got = call()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            twice = [2 * t for t in got]
+        main.wait_stream(side)
+        kept = [t.clone() for t in got]
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    for w, p, q, r in zip(want, got, twice, kept):
+        assert torch.equal(w, p) and torch.equal(2 * w, q) and torch.equal(w, r)
