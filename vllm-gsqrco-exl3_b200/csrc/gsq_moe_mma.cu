@@ -829,7 +829,7 @@ int moe_mma_serves(int type, int k, bool many) {
 
 // What a tile costs, in 256ths of one of a single token, as seen on the blocks of layers with groups of different sizes. In 16ths, the shares of few
 // experts' blocks were as coarse as a share (27 tokens of 8 experts: 88 us, 74 in 256ths). Q6_K's form for two tokens is dear: with the
-// others' rates the blocks of such groups were done at 33 us, those of single tokens at 28 (8 tokens, half of 64 experts: 56 us, 53 with its
+// others' rates the blocks of such groups were done at 33 us, those of single tokens at 28 (8 tokens, a rank's 64 of 128 experts: 56 us, 53 with its
 // own).
 void moe_mma_rates(int type, int (&rate)[5]) {
   static const int rates[2][5] = {{256, 272, 288, 320, 416}, {256, 320, 305, 305, 380}};
