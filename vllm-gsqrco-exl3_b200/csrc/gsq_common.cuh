@@ -67,6 +67,15 @@ __device__ __forceinline__ uint4 ldg_stream_v4(const void* p) {
                : "l"(p));
   return v;
 }
+// The same for what the kernel before may still be writing when this one starts (programmatic launch; after griddepcontrol.wait): such data is
+// not read-only for the kernel's lifetime, so the non-coherent path above is not valid for it.
+__device__ __forceinline__ uint4 ld_stream_v4(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
 __device__ __forceinline__ uint2 ldg_stream_v2(const void* p) {
   uint2 v;
   asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));

@@ -313,7 +313,7 @@ struct Part {
   __device__ __forceinline__ int unit(int u, float (&f)[Vec<T>::N], int& at) const {
     const int nv = v1 - v0;
     if (u >= 1 && u <= nv) {
-      Vec<T>::get(ldg_stream_v4(body + (int64_t)(v0 + u - 1) * Vec<T>::N), f);
+      Vec<T>::get(ld_stream_v4(body + (int64_t)(v0 + u - 1) * Vec<T>::N), f);
       at = body_at + (v0 + u - 1) * Vec<T>::N;
       return Vec<T>::N;
     }
@@ -526,12 +526,12 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobAr
   auto fetch = [&](int v) {
     if (v + (U - 1) * LP_THREADS < p.v1) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) next[u] = ldg_stream_v4(p.body + (int64_t)(v + u * LP_THREADS) * N);
+      for (int u = 0; u < U; ++u) next[u] = ld_stream_v4(p.body + (int64_t)(v + u * LP_THREADS) * N);
     } else {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         next[u] = make_uint4(Vec<T>::MASKED, Vec<T>::MASKED, Vec<T>::MASKED, Vec<T>::MASKED);
-        if (v + u * LP_THREADS < p.v1) next[u] = ldg_stream_v4(p.body + (int64_t)(v + u * LP_THREADS) * N);
+        if (v + u * LP_THREADS < p.v1) next[u] = ld_stream_v4(p.body + (int64_t)(v + u * LP_THREADS) * N);
       }
     }
   };
@@ -661,7 +661,7 @@ __global__ void __launch_bounds__(LPW_WARPS * 32) logprobs_rows_kernel(const Log
 #pragma unroll
   for (int u = 0; u < LPW_VECTORS; ++u) {
     r[u / H][u % H] = make_uint4(Vec<T>::MASKED, Vec<T>::MASKED, Vec<T>::MASKED, Vec<T>::MASKED);
-    if (lane + 32 * u < vectors) r[u / H][u % H] = ldg_stream_v4(x + head + (lane + 32 * u) * N);
+    if (lane + 32 * u < vectors) r[u / H][u % H] = ld_stream_v4(x + head + (lane + 32 * u) * N);
   }
   const int64_t id64 = a.ids[row];
   // a lane's single value: of the head (lanes 0 ..) or of the tail (lanes 16 ..)
