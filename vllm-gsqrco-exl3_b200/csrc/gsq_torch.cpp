@@ -430,11 +430,15 @@ std::tuple<Tensor, std::optional<Tensor>> silu_mul_quantize(const Tensor& gate_u
 
 // ---- mixture-of-experts layer (gsq_b200.quantization.fused_moe) and log probabilities (gsq_b200.logprobs)
 
-// These ops have no backward pass: a call that would need one says so instead of returning a result without a gradient.
-void no_gradient(const char* op, std::initializer_list<const Tensor*> ts) {
-  if (!at::GradMode::is_enabled()) return;
-  for (const Tensor* t : ts)
-    TORCH_CHECK(!t->defined() || !t->requires_grad(), op, ": no gradient is computed here; detach the input or call under torch.no_grad()");
+// These ops have no derivative: a call that would need one says so instead of returning a result without it. (A tangent is there under
+// torch.no_grad() too; torch.inference_mode() hides it.)
+void no_gradient(const char* op, c10::ArrayRef<const Tensor*> ts) {
+  for (const Tensor* t : ts) {
+    if (!t->defined()) continue;
+    TORCH_CHECK(!at::GradMode::is_enabled() || !t->requires_grad(), op,
+                ": no gradient is computed here; detach the input or call under torch.no_grad()");
+    TORCH_CHECK(!t->_fw_grad(0).defined(), op, ": no forward-mode derivative is computed here; detach the input");
+  }
 }
 
 gsq_moe moe_weights(const char* op, const Tensor& x, const Tensor& w13, const Tensor& w2, int64_t t13, int64_t t2, int64_t activation) {
@@ -569,6 +573,31 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& 
   return {lp, rank, entropy, top, top_ids};
 }
 
+// The same refusal where the dispatcher still sees what a derivative is taken of: a transform of functions (torch.func) hands the
+// implementation plain tensors.
+void derivative_of(std::vector<const Tensor*>& ts, const Tensor& t) { ts.push_back(&t); }
+void derivative_of(std::vector<const Tensor*>& ts, const std::optional<Tensor>& t) { if (t) ts.push_back(&*t); }
+template <typename T>
+void derivative_of(std::vector<const Tensor*>&, const T&) {}
+
+template <typename Op, typename F = decltype(Op::run)>
+struct Refusing;
+template <typename Op, typename R, typename... A>
+struct Refusing<Op, R (*const)(A...)> {
+  static R call(A... args) {
+    std::vector<const Tensor*> ts;
+    (derivative_of(ts, args), ...);
+    no_gradient(Op::name, ts);
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow((std::string("_C_gguf::") + Op::name).c_str(), "").template typed<R(A...)>();
+    const at::AutoDispatchBelowAutograd below;
+    return op.call(args...);
+  }
+};
+struct MoeExpertsOp { static constexpr const char* name = "gsq_moe_experts"; static constexpr auto run = &moe_experts; };
+struct MoeLayerOp { static constexpr const char* name = "gsq_moe_layer"; static constexpr auto run = &moe_layer; };
+struct MoeRouteOp { static constexpr const char* name = "gsq_moe_route"; static constexpr auto run = &moe_route; };
+struct TokenLogprobsOp { static constexpr const char* name = "gsq_token_logprobs"; static constexpr auto run = &token_logprobs; };
+
 // ---- registration. The ops are defined in Python (which leaves names alone that another extension has defined); the
 // implementations are added here, one library object per (namespace, key) kept for the process's life.
 
@@ -611,6 +640,13 @@ void implement(const std::string& name) {
     else if (name == "gsq_token_logprobs") l.impl(n, &token_logprobs);
     else TORCH_CHECK(false, "no implementation of ", name);
   }
+  auto refusing = [&](auto op) {
+    if (name == op.name) library("_C_gguf", c10::DispatchKey::Autograd).impl(op.name, &Refusing<decltype(op)>::call);
+  };
+  refusing(MoeExpertsOp());
+  refusing(MoeLayerOp());
+  refusing(MoeRouteOp());
+  refusing(TokenLogprobsOp());
 }
 
 void implement_vllm(const std::string& name) {
