@@ -44,3 +44,45 @@ def test_transforms_of_functions(name):
         torch.func.grad(f)(torch.zeros(shape))
     with pytest.raises(RuntimeError, match="no forward-mode derivative"):
         torch.func.jvp(f, (torch.zeros(shape),), (torch.ones(shape),))
+
+
+class _Head:
+    """A linear method whose product, as the native ones, leaves no trace of a derivative."""
+
+    calls = 0
+
+    def apply(self, layer, x):
+        self.calls += 1
+        return torch.zeros(x.shape[0], layer.weight.shape[0])
+
+
+def test_head_in_front():
+    """The product in front of the log probabilities has no autograd node: its result does not say that x needs a derivative."""
+    layer, head, ids = torch.nn.Module(), _Head(), torch.zeros(3, dtype=torch.int64)
+    layer.weight = torch.nn.Parameter(torch.zeros(100, 144, dtype=torch.uint8), requires_grad=False)
+
+    def call(x):
+        return logprobs.head_logprobs(head, layer, x, ids, 2)
+
+    with pytest.raises(RuntimeError, match="no gradient"):
+        call(torch.zeros(3, 256, requires_grad=True))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        torch.func.grad(lambda x: call(x).logprobs.sum())(torch.zeros(3, 256))
+    with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        torch.func.jvp(lambda x: call(x).logprobs, (torch.zeros(3, 256),), (torch.ones(3, 256),))
+    with fwd.dual_level(), torch.no_grad(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        call(fwd.make_dual(torch.zeros(3, 256), torch.ones(3, 256)))
+    assert head.calls == 0
+    with torch.no_grad(), pytest.raises(RuntimeError, match="must be CUDA"):
+        call(torch.zeros(3, 256, requires_grad=True))
+    assert head.calls == 1
+
+
+def test_head_in_front_traced():
+    layer, head, ids = torch.nn.Module(), _Head(), torch.zeros(3, dtype=torch.int64)
+    layer.weight = torch.nn.Parameter(torch.zeros(100, 144, dtype=torch.uint8), requires_grad=False)
+    call = torch.compile(lambda x: logprobs.head_logprobs(head, layer, x, ids, 2), backend="eager", fullgraph=True)
+    with pytest.raises(RuntimeError, match="must be CUDA"):
+        call(torch.zeros(3, 256))
+    with pytest.raises(Exception, match="no gradient"):
+        call(torch.zeros(3, 256, requires_grad=True))

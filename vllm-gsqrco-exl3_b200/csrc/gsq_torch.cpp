@@ -672,6 +672,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("moe_layer", &moe_layer, free_interpreter());
   m.def("moe_route", &moe_route, free_interpreter());
   m.def("token_logprobs", &token_logprobs, free_interpreter());
+  // (of a step in front whose product leaves no trace of a derivative: logprobs.head_logprobs)
+  m.def("no_gradient", [](const std::string& op, const Tensor& t) { no_gradient(op.c_str(), {&t}); });
   m.def("route", [](int64_t n, int64_t type, int64_t rows, int64_t k, bool packed) -> std::optional<std::string> {
     const int op = route(n, type, rows, k, packed);
     return op < 0 ? std::nullopt : std::optional<std::string>(kSpec[op].name);

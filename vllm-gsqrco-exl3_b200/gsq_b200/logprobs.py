@@ -37,6 +37,11 @@ def head_logprobs(method, layer: torch.nn.Module, x: torch.Tensor, token_ids: to
     rows = x.shape[0]
     if token_ids.dim() != 1 or token_ids.shape[0] != rows:
         raise RuntimeError(f"head_logprobs: token_ids must be [{rows}]")
+    # the product has no autograd node: its result would not say that x needs a derivative
+    if not torch.compiler.is_compiling():
+        _gsq_ops.no_gradient("head_logprobs", x)
+    elif x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("head_logprobs: no gradient is computed here; detach the input or call under torch.no_grad()")
     vocab = layer.weight.shape[0]
     step = max(1, max_logit_bytes // max(1, vocab * x.element_size()))
     parts = [token_logprobs(method.apply(layer, x[i:i + step]), token_ids[i:i + step], top_n) for i in range(0, max(rows, 1), step)]
