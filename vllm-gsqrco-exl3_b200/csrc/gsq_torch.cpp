@@ -575,24 +575,50 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& 
 
 // The same refusal where the dispatcher still sees what a derivative is taken of: a transform of functions (torch.func) hands the
 // implementation plain tensors.
-void derivative_of(std::vector<const Tensor*>& ts, const Tensor& t) { ts.push_back(&t); }
-void derivative_of(std::vector<const Tensor*>& ts, const std::optional<Tensor>& t) { if (t) ts.push_back(&*t); }
+using Tensors = c10::SmallVector<const Tensor*, 8>;
+void tensors_of(Tensors& ts, const Tensor& t) { ts.push_back(&t); }
+void tensors_of(Tensors& ts, const std::optional<Tensor>& t) { if (t) ts.push_back(&*t); }
 template <typename T>
-void derivative_of(std::vector<const Tensor*>&, const T&) {}
+void tensors_of(Tensors&, const T&) {}
+
+template <typename Op, typename R, typename... A>
+const c10::TypedOperatorHandle<R(A...)>& handle_of(R (*)(A...)) {
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow((std::string("_C_gguf::") + Op::name).c_str(), "").template typed<R(A...)>();
+  return op;
+}
 
 template <typename Op, typename F = decltype(Op::run)>
 struct Refusing;
 template <typename Op, typename R, typename... A>
 struct Refusing<Op, R (*const)(A...)> {
   static R call(A... args) {
-    std::vector<const Tensor*> ts;
-    (derivative_of(ts, args), ...);
+    Tensors ts;
+    (tensors_of(ts, args), ...);
     no_gradient(Op::name, ts);
-    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow((std::string("_C_gguf::") + Op::name).c_str(), "").template typed<R(A...)>();
     const at::AutoDispatchBelowAutograd below;
-    return op.call(args...);
+    return handle_of<Op>(Op::run).call(args...);
   }
 };
+
+// Something has to see the call: a transform of functions (torch.func) or a trace on this thread, or a tensor with a dispatch of its own.
+bool seen_by_others(const Tensors& ts) {
+  const auto on = c10::impl::tls_local_dispatch_key_set().included_;
+  if (on.has(c10::DispatchKey::FuncTorchDynamicLayerFrontMode) || on.has(c10::DispatchKey::Tracer)) return true;
+  return std::any_of(ts.begin(), ts.end(), [](const Tensor* t) { return t->defined() && t->unsafeGetTensorImpl()->is_python_dispatch(); });
+}
+// The entry points' native call: straight to the implementation, past the dispatcher, or to the op.
+template <typename Op, typename F = decltype(Op::run)>
+struct Direct;
+template <typename Op, typename R, typename... A>
+struct Direct<Op, R (*const)(A...)> {
+  static R call(A... args) {
+    Tensors ts;
+    (tensors_of(ts, args), ...);
+    if (!seen_by_others(ts)) return Op::run(args...);
+    return handle_of<Op>(Op::run).call(args...);
+  }
+};
+
 struct MoeExpertsOp { static constexpr const char* name = "gsq_moe_experts"; static constexpr auto run = &moe_experts; };
 struct MoeLayerOp { static constexpr const char* name = "gsq_moe_layer"; static constexpr auto run = &moe_layer; };
 struct MoeRouteOp { static constexpr const char* name = "gsq_moe_route"; static constexpr auto run = &moe_route; };
@@ -668,10 +694,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         free_interpreter());
   m.def("rmsnorm_quantize", &rmsnorm_quantize, free_interpreter());
   m.def("silu_mul_quantize", &silu_mul_quantize, free_interpreter());
-  m.def("moe_experts", &moe_experts, free_interpreter());
-  m.def("moe_layer", &moe_layer, free_interpreter());
-  m.def("moe_route", &moe_route, free_interpreter());
-  m.def("token_logprobs", &token_logprobs, free_interpreter());
+  m.def("moe_experts", &Direct<MoeExpertsOp>::call, free_interpreter());
+  m.def("moe_layer", &Direct<MoeLayerOp>::call, free_interpreter());
+  m.def("moe_route", &Direct<MoeRouteOp>::call, free_interpreter());
+  m.def("token_logprobs", &Direct<TokenLogprobsOp>::call, free_interpreter());
   // (of a step in front whose product leaves no trace of a derivative: logprobs.head_logprobs)
   m.def("no_gradient", [](const std::string& op, const Tensor& t) { no_gradient(op.c_str(), {&t}); });
   m.def("route", [](int64_t n, int64_t type, int64_t rows, int64_t k, bool packed) -> std::optional<std::string> {

@@ -24,7 +24,8 @@ SCORINGS = {"softmax": 0, "sigmoid": 1}
 
 
 def _direct(x: torch.Tensor) -> bool:
-    """A plain CUDA tensor and nobody tracing or intercepting: straight to the native code under the custom ops."""
+    """A plain CUDA tensor and nobody compiling or intercepting: straight to the native code under the custom ops, which goes back to
+    the op where torch.func or a jit trace has to see it."""
     return type(x) is torch.Tensor and x.is_cuda and not torch.compiler.is_compiling() and not torch._C._len_torch_dispatch_stack()
 
 
