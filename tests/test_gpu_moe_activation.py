@@ -33,7 +33,7 @@ def _rows(name, scales):
 
 @pytest.mark.parametrize("name", ["Q6_K", "Q2_K"])     # the tensor-core products, the dp4a ones
 @pytest.mark.parametrize("m", [1, 3])
-@pytest.mark.parametrize("act,gates", [("gelu", (0.5, 2, 4, 5, 6, 8, 12)), ("silu", (0.5, 4, 20, 60, 87))])
+@pytest.mark.parametrize("act,gates", [("gelu", (0.5, 2, 4, 5, 6, 8, 12)), ("silu", (0.5, 4, 20, 60, 87, 87.75, 88, 88.5))])
 def test_strongly_negative_gates(name, m, act, gates):
     t = {**synth.TYPE_IDS, **synth.LOW_BIT_TYPE_IDS}[name]
     sign = np.where(np.random.default_rng(1).random(I) < 0.5, -1.0, 1.0)
