@@ -6,8 +6,8 @@ import pytest
 import torch
 
 import gsq_b200  # noqa: F401
-from gsq_b200 import logprobs, synth
-from gsq_b200.quantization import linear
+from gsq_b200 import fused, logprobs, synth
+from gsq_b200.quantization import fused_moe, linear
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -54,5 +54,46 @@ def test_head_then_log_probabilities(name, m):
         part = logprobs.token_logprobs(z[:, :2000], ids[i] % 2000, 3)      # a warp a row
         sync()
         return (*whole, *part)
+
+    _same_without_synchronisation(rounds, step)
+
+
+def _stack(name, experts, rows, k, seed):
+    """[experts, rows, bytes], rows of 2048 at most repeated; values of about 0.02."""
+    raw = torch.from_numpy(synth.make_weight(TYPES[name], min(experts * rows, 2048), k, seed)).to(DEV)
+    w = raw[torch.arange(experts * rows, device=DEV) % len(raw)].view(experts, rows, -1).contiguous()
+    b = w.view(experts, rows, k // 256, -1)
+    for i in {"Q6_K": (208,), "Q4_K": (0, 2)}.get(name, (0,)):
+        b[..., i:i + 2] = (b[..., i:i + 2].contiguous().view(torch.float16).float() * 0.01).to(torch.float16).view(torch.uint8)
+    return w
+
+
+# one token to more than one block of the plan makes the choice for, and more than a pass; products on the tensor cores and by dp4a
+@pytest.mark.parametrize("m,t13,t2", [(1, "Q4_K", "Q6_K"), (4, "IQ4_XS", "Q4_K"), (9, "IQ2_S", "IQ4_XS"), (16, "Q4_K", "IQ2_S"), (70, "Q6_K", "Q4_K"),
+                                      (1040, "Q4_K", "Q4_K")])
+def test_layers_of_norm_router_experts(m, t13, t2):
+    """Fused norm with its residual in place -> router (a quantised linear) -> experts -> the next layer's norm: each reads what the
+    one before it writes after letting it start."""
+    hidden, inter, experts, top_k, layers, rounds = 2048, 512, 16, 3, 3, 6
+    g = torch.Generator(device=DEV).manual_seed(m)
+    gates = [_linear(name, experts, hidden, 20 + i) for i, name in enumerate(("Q6_K", "Q4_K", "IQ3_S"))]
+    w13, w2 = _stack(t13, experts, 2 * inter, hidden, 3), _stack(t2, experts, hidden, inter, 4)
+    gamma = (1 + 0.1 * torch.randn(hidden, device=DEV, generator=g)).to(torch.bfloat16)
+    starts = [torch.randn(m, hidden, device=DEV, generator=g).to(torch.bfloat16) for _ in range(rounds)]
+    residual = torch.empty_like(starts[0])
+
+    def step(i, sync):
+        x = starts[i]
+        residual.zero_()
+        for layer, method in gates[:layers]:
+            _, y = fused.rmsnorm_quantize_q8_1(x, gamma, 1e-6, residual, want_y=True)
+            sync()
+            z = method.apply(layer, y)
+            sync()
+            x = fused_moe.moe_layer_gguf(y, z, w13, w2, TYPES[t13], TYPES[t2], top_k)
+            sync()
+        _, last = fused.rmsnorm_quantize_q8_1(x, gamma, 1e-6, residual, want_y=True)
+        sync()
+        return x, last, residual.clone()
 
     _same_without_synchronisation(rounds, step)
