@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(128) moe_route_kernel(const RouteArgs a) {
 }
 
 static int launch_route(const RouteArgs& a, cudaStream_t st) {
-  const unsigned grid = (unsigned)((a.m + 3) / 4);
+  const unsigned grid = (unsigned)(((int64_t)a.m + 3) / 4);
   if (a.experts <= 64) moe_route_kernel<2><<<grid, 128, 0, st>>>(a);
   else if (a.experts <= 256) moe_route_kernel<8><<<grid, 128, 0, st>>>(a);
   else moe_route_kernel<ROUTE_PER_LANE><<<grid, 128, 0, st>>>(a);
