@@ -373,8 +373,9 @@ int gsq_peer_reduce_error_flag(int* flag);
  *                    calls that may overlap
  * gsq_moe_route: the choice alone. logits [m, experts] in `dtype`; scoring GSQ_MOE_SOFTMAX or _SIGMOID; the top_k largest
  *   logits, or largest score + bias [experts] where bias is not NULL, ties to the lowest number; weight = score (divided by
- *   the sum of the chosen ones where renormalize != 0) * scale. An expert with logit -inf or NaN is never chosen; a choice that
- *   finds none left is id -1, weight 0. Experts at +inf share the weight.
+ *   the sum of the chosen ones where renormalize != 0) * scale. An expert with logit, or score + bias, -inf or NaN is never chosen; a choice
+ *   that finds none left is id -1, weight 0. Experts at +inf share the weight. Scores are fp32: a sigmoid of a logit below -88 is 0, and where all
+ *   chosen scores are 0 so are the weights.
  * gsq_moe_layer: gsq_moe_route and gsq_moe_experts in one call, ids and weights kept in the workspace.
  * Limits: experts <= 1024, top_k <= 32, m <= 65536, hidden and inter <= 131072 (GSQ_ERR_TOO_LARGE).
  */
@@ -412,7 +413,8 @@ int gsq_moe_layer(const gsq_moe* w, const void* x, int x_dtype, int64_t m, int64
  * What a server answers with behind the head: per row of logits [m, vocab] (dtype, rows row_stride elements apart) the log
  * probability of one given token, its rank, the row's entropy and the top_n (0..32) most probable tokens with their log
  * probabilities. Pointers aligned to their elements. Not in the reference (vLLM's sampler runs log_softmax, gather, a comparison and topk). Natural logarithms,
- * statistics in fp32. Order of tokens: larger logit first, lower index first among equals, NaN last.
+ * statistics in fp32. Order of tokens: larger logit first, lower index first among equals, NaN last (a rank that counts all logits >= the
+ * token's, as samplers have it, is larger behind equal ones).
  *   token_ids      [m] int64. Negative: no token (log probability 0, rank 0). >= vocab: NaN, rank 0.
  *   logprobs [m], ranks [m] (1 = first in that order), entropy [m]
  *   top_logprobs, top_ids   [m, top_n]; NULL where top_n = 0. Past the vocabulary: -inf, id -1.

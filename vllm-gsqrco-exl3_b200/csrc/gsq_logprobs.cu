@@ -7,7 +7,8 @@
 // A row is cut over a cluster of 1 .. 16 blocks, so that a few rows use the whole GPU, and the parts meet in shared memory:
 // no workspace, one launch. Rows of at most 256 whole vectors take a warp each.
 //
-// Measured (bf16): 2048 rows of 248320 values with 5 alternatives 182 us, 5.6 TB/s (0.86 of the measured 6.54; 165 us without rank and alternatives);
+// Measured (bf16): 2048 rows of 248320 values with 5 alternatives 187 us in the first 20 ms, 5.4 TB/s (0.83 of the measured 6.54), and 207 in the long run, 4.9 TB/s, when the
+// card holds its power limit;
 // 512 rows of 151936 37 us: some SMs have four rows, others three, and an SM goes through its rows at 32 B/ns at most; one row of 248320, 20 alternatives, 9.4 us, all of it latency: loads 1.5, alternatives 2.5, joining the cluster 3.5, launch 2.
 //
 // Alternatives: the threads' maxima, gathered to 32 groups, give a value that at least top_n values of the block's part reach
@@ -642,7 +643,8 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(const LogprobAr
 }
 
 // Rows of at most 256 whole vectors: a warp a row, the row in registers, no barrier. With a block a row, 4096 rows of 1000 fp32 logits
-// took 46 us: a row's fixed steps outweigh its 4 KB.
+// took 46 us: a row's fixed steps outweigh its 4 KB. Here 11.7 us (2048 rows 8.5): 80 registers leave three blocks an SM, so that 512 blocks go in two
+// waves. In bf16 (160 registers, one block an SM) 18.8. Longer rows pay the block's steps: 1028 values 45.4, 4096 values 48.1.
 constexpr int LPW_WARPS = 8, LPW_VECTORS = 8, LPW_ROOM = 128;
 
 template <typename T>
@@ -778,7 +780,8 @@ static int launch_logprobs(const LogprobArgs& a, int64_t m, cudaStream_t st) {
   const int rc = device_info(&di);
   if (rc != GSQ_OK) return rc;
   const void* kern = (const void*)logprobs_kernel<T>;
-  // blocks of a row: as many as leave every block at least one round of loads, while the grid stays within two blocks an SM
+  // blocks of a row: doubled while that leaves every block half a round of loads or more and the grid within two blocks an SM. One row with 0 (20) alternatives, so and with
+  // a whole round at least: 16400 values 4.5, 4.9 us (8.2, 8.6), 64000 4.6, 5.1 (8.5, 8.9), 151936 5.4, 5.5 (9.5, 9.4); of a single round the other is the better, 8193 values 4.4, 3.7 (8.2, 6.1)
   const int64_t rounds = (a.vocab / Vec<T>::N) / (LP_THREADS * LP_UNROLL);
   int cs = 1;
   while (cs < 16 && 2 * cs * m <= 2 * di.sm_count && cs <= rounds) cs *= 2;

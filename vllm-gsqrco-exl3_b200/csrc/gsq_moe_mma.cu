@@ -14,9 +14,10 @@
 //     the order of the tensor-core instruction's B fragment. An instruction takes the 8 columns from its group's first on; what it finds
 //     past the group's own only reaches sums that are not stored. A group of more than 8 takes two instructions on one decoding.
 //   * Product: mma.sync m16n8k32 on bytes (m16n8k16 for Q6_K, whose sub-scales cover 16 values); a lane decodes exactly its share of
-//     the A fragment. tcgen05 has no 8-bit integer form, and every 32 values' sums are scaled on their own before they are added, which
-//     would read an accumulator out of TMEM once per slice. That scaling, not the instruction, is the cost: with a column for
-//     each of 8 tokens it is 14 instructions a slice and lane. A group of 1, 2 or 4 tokens therefore gives the free columns to other
+//     the A fragment. (tcgen05.mma has an 8-bit integer form, kind::i8, but 128 rows to an instruction and an accumulator that is read out of
+//     TMEM once per slice, since every 32 values' sums are scaled on their own before they are added: gsq_gemm5.cuh does that for many
+//     columns, and the linear path takes it from 33 rows on. Experts with more than 16 tokens could use it; here they decode their weights once
+//     for every 16.) That scaling, not the instruction, is the cost: with a column for each of 8 tokens it is 14 instructions a slice and lane. A group of 1, 2 or 4 tokens therefore gives the free columns to other
 //     slices: the instruction of slice j has the activations in the columns of slice j and zeros in the others, and the sums of 8, 4
 //     or 2 slices come out side by side in one C fragment, scaled at once.
 //   * Sums leave the instruction on the bit pattern of 1.5 * 2^23, so fma(sum, dA, -1.5 * 2^23 dA) is the exact integer times
@@ -26,9 +27,12 @@
 //   * A tile that several warps have parts of is added up by the warp that has its beginning, in the order of the warps.
 //
 // Measured, 64 experts of 4096 x 2048 with 1, 2, 4, 8, 16 tokens each, the whole layer (least time at the measured 6.54 TB/s in front): Q4_K 138:
-// 171, 174, 186, 220, 308 us; IQ4_XS 131: 266, 269, 296, 333, 405; Q6_K 202: 273, 337, 337, 316, 403; IQ3_S 106: 333, 348, 373, 396, 479. Q4_K
-// with one token an expert runs at DRAM's rate (85 % with the 25 us that a call takes besides); the others are bound by the
-// instructions that decode them (look-ups of 8 nibbles, 6-bit values put together, a codebook).
+// 173, 177, 185, 221, 308 us; IQ4_XS 131: 265, 268, 294, 334, 403; Q6_K 202: 276, 319, 335, 339, 427; IQ3_S 106: 346, 354, 374, 400, 480. Q4_K
+// with one token an expert comes to 80 % of DRAM's rate, 93 % without the 25 us that a call takes besides. IQ4_XS and IQ3_S are bound by the logic pipe, which
+// decodes them (look-ups of 8 nibbles, a codebook with signs): 72 to 81 % busy, the most frequent stall a full pipe, DRAM at 25 to 40 %. Q4_K and Q6_K
+// from a few tokens an expert on fill nothing (logic 37 to 57 %, issue slots 43 to 71 %): dependent instructions with four warps a scheduler, since one
+// kernel with the forms for 1 to 16 tokens takes 126 to 128 registers.
+// Many tokens an expert cost by sixteens: 64 experts of 5120 x 1280, top 8, Q4_K / Q6_K, 64, 256, 1024 tokens: 273, 670, 2278 us.
 #include <type_traits>
 
 #include "gsq_moe.cuh"
@@ -777,8 +781,8 @@ static int kind_of(int type) {
   return type == GSQ_TYPE_Q4_K ? Q4K : type == GSQ_TYPE_Q6_K ? Q6K : type == GSQ_TYPE_IQ3_S ? IQ3S : type == GSQ_TYPE_IQ4_XS ? IQ4XS : -1;
 }
 
-// Columns of activations, superblocks of a stage and stages of a warp's ring beside rows of k values. Where experts have more than 4 pairs on
-// average (`many`), so that some have more than 8, 16 columns come before large stages: 16 tokens on one decoding of the weights (Q4_K,
+// Columns of activations, superblocks of a stage and stages of a warp's ring beside rows of k values. Where experts have more than 4 choices on
+// average (`many`: MoeArgs), so that some have more than 8, 16 columns come before large stages: 16 tokens on one decoding of the weights (Q4_K,
 // 64 experts of 4096 x 2048: 314 us, in groups of 8 430); else the other way round (a token an expert: 171 us, 187 with stages
 // of one superblock). False: too long a row.
 struct Plan {

@@ -2,7 +2,7 @@
 answers with behind the head's product.
 
 The reference leaves this to vLLM's sampler (log_softmax over the logits, a gather, a comparison and a topk, each over the whole
-row); here it is one kernel that reads the logits once. No gradient is computed.
+row); here it is one kernel that reads the logits once. No derivative is computed: a call that would need one is refused.
 """
 
 from __future__ import annotations
@@ -16,7 +16,8 @@ from .quantization.fused_moe import _direct
 
 
 class TokenLogprobs(NamedTuple):
-    """Of each row. A rank of 1 is the most probable token; equal logits rank by index."""
+    """Of each row. A rank of 1 is the most probable token; equal logits rank by index (a sampler that counts all logits >= the token's
+    gives a token behind equal ones, frequent in 16 bits, a larger rank)."""
     logprobs: torch.Tensor       # fp32 [rows]: natural log probability of the given token
     ranks: torch.Tensor          # int64 [rows]
     entropy: torch.Tensor        # fp32 [rows], in nats

@@ -10,7 +10,8 @@ the weighted sum as kernels of their own; here the layer is one call.
 
 Weights are uint8 in GGUF order (not repacked), any of the ten types: w13 [experts, 2 * inter, bytes of `hidden` values] with the
 gate rows before the up rows, w2 [experts, hidden, bytes of `inter` values]; gguf_load.load_experts makes them from a file.
-Activations are taken in 8 bits, 32 values to a scale, as in every product of this package. No gradient is computed.
+Activations are taken in 8 bits, 32 values to a 32-bit scale (the linear path's block_q8_1 has a 16-bit one). No derivative is computed: a call
+that would need one is refused.
 """
 
 from __future__ import annotations
@@ -46,7 +47,8 @@ def fused_moe_gguf(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, topk_we
 def moe_route(router_logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", renormalize: bool = True, bias: torch.Tensor | None = None,
               scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
     """(weights fp32, ids int32), both [tokens, top_k]: the experts of largest score (score + bias [experts] where given), ties to the
-    lowest number. An expert whose logit is -inf or NaN is never chosen; a choice that finds none left has id -1, weight 0."""
+    lowest number. An expert whose logit, or score + bias, is -inf or NaN is never chosen; a choice that finds none left has id -1, weight 0.
+    Scores are 32-bit: a sigmoid of a logit below -88 is 0, and where all chosen scores are 0 so are the weights."""
     sc = _code(SCORINGS, scoring, "scoring")
     return (_gsq_ops.moe_route if _direct(router_logits) else torch.ops._C_gguf.gsq_moe_route)(router_logits, top_k, sc, renormalize, bias, scale)
 
