@@ -32,6 +32,17 @@ def test_native_calls_reach_the_op(name):
     assert any("_C_gguf.gsq_" in s for s in seen), seen
 
 
+def test_native_products_leave_a_transform_to_the_op():
+    w = torch.zeros(256, 144, dtype=torch.uint8)
+    torch.func.vmap(lambda x: _none(_gsq_ops.linear(x, w, 12, None, False), x))(torch.zeros(2, 3, 256))
+    torch.func.vmap(lambda x: _none(_gsq_ops.linear_runs(x, w, [0, 256, 144, 12], False), x))(torch.zeros(2, 3, 256))
+
+
+def _none(out, x):
+    assert out is None
+    return x
+
+
 def _stacks():
     import numpy as np
 
@@ -80,3 +91,43 @@ def test_jit_trace():
     for _ in range(2):
         args = new()
         assert all(torch.equal(p, q) for p, q in zip(traced(*args), f(*args)))
+
+
+def _head(vocab=9000, k=512, name="Q6_K"):
+    from gsq_b200.quantization import linear
+
+    layer, method = torch.nn.Module(), linear.GGUFLinearMethod(None)
+    method.create_weights(layer, k, [vocab], k, vocab, torch.bfloat16)
+    layer.weight.load_shard(torch.from_numpy(synth.make_weight(synth.TYPE_IDS[name], vocab, k, 5)).cuda(), None)
+    layer.weight_type.weight_type = synth.TYPE_IDS[name]
+    method.process_weights_after_loading(layer)
+    return layer, method
+
+
+@pytest.mark.gpu
+@pytest.mark.filterwarnings("ignore")
+def test_head_under_vmap_trace_and_compile():
+    g = torch.Generator(device="cuda").manual_seed(6)
+    layer, method = _head()
+    w13, w2 = _stacks()
+    ids = torch.randint(0, 9000, (5,), device="cuda", generator=g)
+    new = lambda: (torch.randn(5, 512, device="cuda", generator=g).to(torch.bfloat16), torch.randn(5, 4, device="cuda", generator=g))  # noqa: E731
+
+    def f(x, z):
+        m = fused_moe.moe_layer_gguf(x, z, w13, w2, 12, 14, 2)
+        y = x + 1e-3 * m
+        return (m, y, *logprobs.head_logprobs(method, layer, y, ids, 3))
+
+    pairs = [new() for _ in range(3)]
+    got = torch.func.vmap(f)(torch.stack([x for x, _ in pairs]), torch.stack([z for _, z in pairs]))
+    want = [f(*p) for p in pairs]
+    for i, t in enumerate(got):
+        assert torch.equal(t, torch.stack([w[i] for w in want]))
+    traced = torch.jit.trace(f, new(), check_trace=False)
+    compiled = torch.compile(f, backend="aot_eager", fullgraph=True)
+    for call in (traced, compiled):
+        for p, w in zip(pairs, want):
+            m, y, *got = call(*p)
+            # (y itself may be rounded once there where it is rounded twice here: a trace fuses its two steps)
+            assert torch.equal(m, w[0])
+            assert all(torch.equal(a, b) for a, b in zip(got, logprobs.head_logprobs(method, layer, y, ids, 3)))

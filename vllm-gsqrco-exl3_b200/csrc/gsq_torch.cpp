@@ -601,7 +601,7 @@ struct Refusing<Op, R (*const)(A...)> {
 };
 
 // Something has to see the call: a transform of functions (torch.func) or a trace on this thread, or a tensor with a dispatch of its own.
-bool seen_by_others(const Tensors& ts) {
+bool seen_by_others(c10::ArrayRef<const Tensor*> ts) {
   const auto on = c10::impl::tls_local_dispatch_key_set().included_;
   if (on.has(c10::DispatchKey::FuncTorchDynamicLayerFrontMode) || on.has(c10::DispatchKey::Tracer)) return true;
   return std::any_of(ts.begin(), ts.end(), [](const Tensor* t) { return t->defined() && t->unsafeGetTensorImpl()->is_python_dispatch(); });
@@ -689,8 +689,18 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("implement_vllm", &implement_vllm);
   // The calls that launch let go of the interpreter, as the custom ops do: the allocator may wait for the driver in them.
   using free_interpreter = pybind11::call_guard<pybind11::gil_scoped_release>;
-  m.def("linear", &linear, free_interpreter());
-  m.def("linear_runs", [](const Tensor& x, const Tensor& w, const std::vector<int64_t>& runs, bool packed) { return linear_runs(x, w, runs, packed); },
+  // (None where a transform or a trace has to see the call: apply() then takes the op)
+  m.def("linear",
+        [](const Tensor& x, const Tensor& w, int64_t type, const std::optional<Tensor>& x_q8, bool packed) -> std::optional<Tensor> {
+          if (seen_by_others({&x, &w})) return std::nullopt;
+          return linear(x, w, type, x_q8, packed);
+        },
+        free_interpreter());
+  m.def("linear_runs",
+        [](const Tensor& x, const Tensor& w, const std::vector<int64_t>& runs, bool packed) -> std::optional<Tensor> {
+          if (seen_by_others({&x, &w})) return std::nullopt;
+          return linear_runs(x, w, runs, packed);
+        },
         free_interpreter());
   m.def("rmsnorm_quantize", &rmsnorm_quantize, free_interpreter());
   m.def("silu_mul_quantize", &silu_mul_quantize, free_interpreter());

@@ -351,9 +351,13 @@ class GGUFLinearMethod:
         # a plain CUDA tensor and nobody tracing or intercepting: straight to the native code under the custom ops
         direct = type(x) is torch.Tensor and x.is_cuda and not torch.compiler.is_compiling() and not torch._C._len_torch_dispatch_stack()
         if weight_type is not None:
-            out = (_gsq_ops.linear if direct else fused_mul_mat_gguf)(x, weight, weight_type, None, packed)
+            out = _gsq_ops.linear(x, weight, weight_type, None, packed) if direct else None
+            if out is None:      # (also where torch.func or a jit trace has to see the call)
+                out = fused_mul_mat_gguf(x, weight, weight_type, None, packed)
         elif runs is not None:
-            out = (_gsq_ops.linear_runs if direct else torch.ops._C_gguf.gsq_linear_runs)(x, weight, runs, packed)
+            out = _gsq_ops.linear_runs(x, weight, runs, packed) if direct else None
+            if out is None:
+                out = torch.ops._C_gguf.gsq_linear_runs(x, weight, runs, packed)
         else:
             types = layer.weight_type.shard_weight_type
             shard_id = ["q", "k", "v"] if "q" in weight.shard_id else weight.shard_id
