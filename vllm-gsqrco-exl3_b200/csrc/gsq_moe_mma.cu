@@ -30,7 +30,7 @@
 // 173, 177, 185, 221, 308 us; IQ4_XS 131: 265, 268, 294, 334, 403; Q6_K 202: 276, 319, 335, 339, 427; IQ3_S 106: 346, 354, 374, 400, 480. Q4_K
 // with one token an expert comes to 80 % of DRAM's rate, 93 % without the 25 us that a call takes besides. IQ4_XS and IQ3_S are bound by the logic pipe, which
 // decodes them (look-ups of 8 nibbles, a codebook with signs): 72 to 81 % busy, the most frequent stall a full pipe, DRAM at 25 to 40 %. Q4_K and Q6_K
-// from a few tokens an expert on fill nothing (logic 37 to 57 %, issue slots 43 to 71 %): dependent instructions with four warps a scheduler, since one
+// in the layers captured (smaller ones with one token an expert, 8 tokens an expert) fill nothing (logic 37 to 57 %, issue slots 43 to 71 %): dependent instructions with four warps a scheduler, since one
 // kernel with the forms for 1 to 16 tokens takes 126 to 128 registers.
 // Many tokens an expert cost by sixteens: 64 experts of 5120 x 1280, top 8, Q4_K / Q6_K, 64, 256, 1024 tokens: 273, 670, 2278 us.
 #include <type_traits>
